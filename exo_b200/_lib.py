@@ -34,6 +34,15 @@ PROTOTYPES = {
     "ssyrk_exo": [vp, i64, i64, vp, vp],
     "ssyrk_exo_ffma": [vp, i64, i64, vp, vp],
     "ssyrk_exo_3xtf32": [vp, i64, i64, vp, vp],
+    "quantize_rows_bf16_exo": [vp, i64, i64, vp, vp, vp],
+    "quantize_rows_f32_exo": [vp, i64, i64, vp, vp, vp],
+    "gemm_i8_scaled_bf16_exo": [vp, i64, i64, i64] + [vp] * 6,
+    "gemm_i8_scaled_f32_exo": [vp, i64, i64, i64] + [vp] * 6,
+    "linear_i8_bf16_exo": [vp, i64, i64, i64] + [vp] * 7,
+    "linear_i8_f32_exo": [vp, i64, i64, i64] + [vp] * 7,
+    "gated_bf16_exo": [vp, i64, i64, i64, i64] + [vp] * 6,
+    "gated_bf16_backward_exo": [vp, i64, i64, i64, i64] + [vp] * 11,
+    "gated_i8_bf16_exo": [vp, i64, i64, i64, i64] + [vp] * 7,
     # the Gemmini library's "auto" entry points (include/exo_b200_gemmini_shim.h)
     "tiled_matmul_auto": [ctypes.c_size_t] * 3 + [vp] * 4 + [ctypes.c_size_t] * 4 + [ctypes.c_float] * 3
                          + [ctypes.c_int, ctypes.c_float, ctypes.c_float] + [cbool] * 5 + [ctypes.c_uint8, ctypes.c_int],
@@ -46,6 +55,34 @@ for _n in _MM_INSTANCES:
 for _n in _CONV_INSTANCES:
     PROTOTYPES[f"conv_{_n}_cpu"] = [vp, vp, vp, vp, vp, cbool, vp]
     PROTOTYPES[f"conv_{_n}"] = [vp, vp, vp, vp, vp, cbool, vp]
+
+# Element type and shape (as names of the sizes) of every tensor of the feed-forward entry points, in order; "?"
+# marks one that may be None.  The wrapper holds arrays and tensors against these before the call.
+_LINEAR = "M N K", "{t} M K, i8 N K, f32 N, f32? N, i8 M K, f32 M, {t} M N"
+_SCALED = "M N K", "i8 M K, i8 N K, f32 M, f32 N, f32? N, {t} M N"
+
+
+def _signature(sizes, tensors, t=""):
+    specs = []
+    for spec in tensors.format(t=t).split(","):
+        kind, *dims = spec.split()
+        specs.append((kind.rstrip("?"), kind.endswith("?"), tuple(sizes.split().index(d) for d in dims)))
+    return len(sizes.split()), tuple(specs)
+
+
+SIGNATURES = {
+    "quantize_rows_bf16_exo": _signature("M K", "bf16 M K, i8 M K, f32 M"),
+    "quantize_rows_f32_exo": _signature("M K", "f32 M K, i8 M K, f32 M"),
+    "gemm_i8_scaled_bf16_exo": _signature(*_SCALED, "bf16"),
+    "gemm_i8_scaled_f32_exo": _signature(*_SCALED, "f32"),
+    "linear_i8_bf16_exo": _signature(*_LINEAR, "bf16"),
+    "linear_i8_f32_exo": _signature(*_LINEAR, "f32"),
+    "gated_bf16_exo": _signature("act M F K", "bf16 M K, bf16 F K, bf16 F K, bf16 M F, bf16? M F, bf16? M F"),
+    "gated_bf16_backward_exo": _signature(
+        "act M F K", "bf16 M K, bf16 F K, bf16 F K, bf16 M F, bf16 M F, bf16 M F, bf16 M F, bf16 M F, "
+                     "bf16? M K, bf16? F K, bf16? F K"),
+    "gated_i8_bf16_exo": _signature("act M F K", "i8 M K, i8 F K, i8 F K, f32 M, f32 F, f32 F, bf16 M F"),
+}
 
 SUPPORT = {
     "exo_b200_context_create": ([ctypes.c_int, vp], vp),

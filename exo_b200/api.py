@@ -112,6 +112,52 @@ class ProcWrapper:
             raise ExoB200Error(code, self._dll.exo_b200_last_error_string().decode())
 
 
+_KINDS = {"bf16": "bfloat16 int16 uint16", "i8": "int8", "f32": "float32"}  # bf16 travels as 16-bit patterns, too
+_accepted: dict = {}
+
+
+def _dtypes(kind):
+    """The numpy and torch element types that count as ``kind``."""
+    if kind not in _accepted:
+        names = _KINDS[kind].split()
+        found = {np.dtype(n) for n in names if n != "bfloat16"}
+        import sys
+
+        torch = sys.modules.get("torch")
+        if torch is None:
+            return found
+        _accepted[kind] = frozenset(found | {getattr(torch, n) for n in names})
+    return _accepted[kind]
+
+
+class CheckedProc(ProcWrapper):
+    """An entry point whose arrays and tensors are held against its signature (element type, number of elements)
+    before the call: through raw pointers a wrong one would be read or written past its end."""
+
+    def __init__(self, dll, name):
+        super().__init__(dll, name)
+        self._sizes, self._tensors = _lib.SIGNATURES[name]
+
+    def __call__(self, *args, **kwargs):
+        sizes = args[1:1 + self._sizes]
+        tensors = args[1 + self._sizes:]
+        if len(tensors) == len(self._tensors) and all(isinstance(n, (int, np.integer)) for n in sizes):
+            for at, (a, (kind, optional, dims)) in enumerate(zip(tensors, self._tensors), 1):
+                if a is None:
+                    continue  # a NULL that the entry point does not take is its own refusal
+                if not (isinstance(a, np.ndarray) or _is_torch(a)):
+                    raise ValueError(f"{self._name}: operand {at}: unrecognized type {type(a)}")
+                if a.dtype not in _dtypes(kind):
+                    raise ValueError(f"{self._name}: operand {at} holds {a.dtype}, not {kind}")
+                count = 1
+                for d in dims:
+                    count *= int(sizes[d])
+                have = a.size if isinstance(a, np.ndarray) else a.numel()
+                if have != count:
+                    raise ValueError(f"{self._name}: operand {at} has {have} elements, not {count}")
+        super().__call__(*args, **kwargs)
+
+
 class Library:
     """``lib.<proc>(ctxt, ...)`` for every entry point of include/exo_b200.h."""
 
@@ -120,7 +166,7 @@ class Library:
 
     def __getattr__(self, item):
         if item in _lib.PROTOTYPES:
-            w = ProcWrapper(self.dll, item)
+            w = (CheckedProc if item in _lib.SIGNATURES else ProcWrapper)(self.dll, item)
             setattr(self, item, w)
             return w
         raise AttributeError(item)

@@ -304,7 +304,7 @@ std::vector<char> block_upload_order(const BlockPipeline& p) {
   return order;
 }
 
-static bool stream_is_capturing(cudaStream_t s) {
+bool stream_is_capturing(cudaStream_t s) {
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(s, &cap) != cudaSuccess) {
     cudaGetLastError();
@@ -378,7 +378,7 @@ void exo_b200_context_destroy(exo_b200_Context* c) {
   cudaGetDevice(&cur);
   if (cur != c->device) cudaSetDevice(c->device);  // streams, events and allocations are this device's
   cudaStreamSynchronize(c->stream);
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < kStageSlots; i++)
     if (c->stage[i]) cudaFree(c->stage[i]);
   for (int i = 0; i < 3; i++) {
     if (c->scratch[i]) cudaFree(c->scratch[i]);

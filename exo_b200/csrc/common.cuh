@@ -13,6 +13,7 @@
 
 namespace exob200 {
 
+constexpr int kStageSlots = 14;  // operands of the entry point that has most of them
 constexpr uint32_t kContextMagic = 0x45584F42u;  // "EXOB"
 
 // Device-side status word written by kernels whose bounded waits ran out.
@@ -41,8 +42,8 @@ struct exo_b200_Context {
   int sgemm_path;
   int sm_count;
   // grow-only device staging area for host-pointer calls
-  void* stage[4];
-  size_t stage_bytes[4];
+  void* stage[exob200::kStageSlots];
+  size_t stage_bytes[exob200::kStageSlots];
   // device scratch for kernels that need it (repacked operands)
   void* scratch[3];  // 0, 1: per-call operand copies; 2: the split weights of the tensor-core convolution
   size_t scratch_bytes[3];
@@ -120,10 +121,11 @@ struct Operand {
   bool staged;
 };
 
-// Prepares operand `slot` (0..3).  copy_in: contents are needed on the device.
+// Prepares operand `slot` (0 .. kStageSlots - 1).  copy_in: contents are needed on the device.
 bool stage_in(exo_b200_Context* c, int slot, const void* user, size_t bytes, bool copy_in, Operand* op);
 // Copies a staged output back and synchronises; no-op for device pointers.
 bool stage_out(exo_b200_Context* c, const Operand& op);
+bool stream_is_capturing(cudaStream_t s);
 // If any operand was staged the call is synchronous: wait and read the status.
 bool finish(exo_b200_Context* c, bool any_staged);
 

@@ -1,0 +1,75 @@
+// Feed-forward operators (int8 products with token and channel scales, gated projections and their
+// backward pass): what the entry points in ffn_api.cu hand to the kernels.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace exob200 {
+namespace ffn {
+
+enum Kind {
+  SCALED = 0,  // C[M,N] = (A[M,K] B[N,K]^T) * row_scale * col_scale + bias, int8 operands
+  GATED,       // H[M,N] = act(A B0^T) * (A B1^T), bf16; G and U kept on request
+  GATED_I8,    // the same on int8 operands with scales
+  DGRAD,       // C[M,N] = A0[M,K] B0[K,N] + A1[M,K] B1[K,N], bf16
+  WGRAD        // C0[M,N] = A0[K,M]^T B0[K,N], C1 = A1^T B0, bf16
+};
+
+// One product.  M, N: rows and columns of an output; K: the reduction length.  Device pointers.
+struct Problem {
+  int64_t M, N, K;
+  const void *a0, *a1, *b0, *b1;
+  const float *row_scale, *col_scale, *col_scale1, *bias;
+  void *c0, *c1, *c2;
+  int act;
+};
+
+// Both are ordered on the context's stream.
+cudaError_t launch_quantize_rows(exo_b200_Context* ctx, int64_t M, int64_t K, const void* X, bool bf16, int8_t* Q,
+                                 float* scale);
+cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p);
+// dG = dH * U * act'(G), dU = dH * act(G), n elements
+cudaError_t launch_gate_backward(exo_b200_Context* ctx, int act, int64_t n, const uint16_t* G, const uint16_t* U,
+                                 const uint16_t* dH, uint16_t* dG, uint16_t* dU);
+
+// ------------------------------------------------------------------ activations
+// All three are g * p(g) with p the logistic function of g, the normal distribution function, or the logistic
+// function of twice the tanh argument ((1 + tanh z) / 2 = 1 / (1 + exp(-2 z))).  The fast exponential and
+// division are good to a few units of 2^-22 here, far inside the bf16 rounding of every result.
+__device__ __forceinline__ float logistic(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+constexpr float kRootHalf = 0.70710678f;      // sqrt(1 / 2)
+constexpr float kRoot2Pi = 0.79788456f;       // sqrt(2 / pi)
+constexpr float kTanhCubic = 0.044715f;
+// beyond this p is 0 or 1 in fp32 for the two GELUs; keeps the cubic and its derivative finite
+constexpr float kGeluClamp = 32.0f;
+
+template <int ACT>
+__device__ __forceinline__ float gate_p(float g) {
+  if (ACT == EXO_B200_ACT_SILU) return logistic(g);
+  if (ACT == EXO_B200_ACT_GELU) return 0.5f * erfcf(-kRootHalf * g);
+  const float c = fminf(fmaxf(g, -kGeluClamp), kGeluClamp);
+  return logistic(2.0f * kRoot2Pi * (c + kTanhCubic * c * c * c));
+}
+template <int ACT>
+__device__ __forceinline__ float gate(float g) {
+  return g * gate_p<ACT>(g);
+}
+// derivative of g p(g), given p
+template <int ACT>
+__device__ __forceinline__ float gate_slope(float g, float p) {
+  if (ACT == EXO_B200_ACT_SILU) return p * (1.0f + g * (1.0f - p));
+  if (ACT == EXO_B200_ACT_GELU) return p + g * __expf(-0.5f * g * g) * (0.5f * kRoot2Pi);
+  const float c = fminf(fmaxf(g, -kGeluClamp), kGeluClamp);
+  return p + c * p * (1.0f - p) * (2.0f * kRoot2Pi) * (1.0f + 3.0f * kTanhCubic * c * c);
+}
+
+__device__ __forceinline__ float scaled(int32_t acc, float row, float col) {
+  return __int2float_rn(acc) * row * col;
+}
+
+}  // namespace ffn
+}  // namespace exob200

@@ -208,6 +208,59 @@ void ssyrk_exo_ffma( void *ctxt, int_fast32_t N, int_fast32_t K, const float* A,
 void ssyrk_exo_3xtf32( void *ctxt, int_fast32_t N, int_fast32_t K, const float* A, float* C );
 
 /* ------------------------------------------------------------------------
+ * Feed-forward blocks of language models: 8-bit products with a scale for each
+ * token (row) and each channel (column), and gated projections, forward and
+ * backward.  Same conventions as gemm_bf16_exo: bf16 travels as uint16_t, every
+ * weight matrix is column-major K x N, i.e. one output channel per row of an
+ * [N, K] array, tensors are dense and do not alias, sizes are >= 1, pointers are
+ * host or device memory and aligned to their element.  bool / enum arguments by value.
+ * A call whose operands are all device memory only enqueues and may be captured
+ * into a CUDA graph (operand copies that an unaligned pitch needs live in
+ * stream-ordered memory that belongs to the call, in a graph to the graph); a call
+ * with host operands on a capturing stream is refused (EXO_B200_ERR_UNSUPPORTED).
+ * --------------------------------------------------------------------- */
+
+/* quantize_rows_*_exo: one scale for each row of X.  top = max_k |X[i,k]|:
+ *   scale[i] = top / 127;   Q[i,k] = the integer nearest to X[i,k] * (127 / top), ties to even
+ * (both quotients rounded to fp32, the product not rounded before it goes to an integer).  A row of
+ * zeros gets scale 0 and zeros; a row that holds an infinity or a NaN gets scale NaN and zeros, so
+ * that every product with it is NaN. */
+void quantize_rows_bf16_exo( void *ctxt, int_fast32_t M, int_fast32_t K, const uint16_t* X, int8_t* Q, float* scale );
+void quantize_rows_f32_exo( void *ctxt, int_fast32_t M, int_fast32_t K, const float* X, int8_t* Q, float* scale );
+
+/* gemm_i8_scaled_*_exo: C[i,j] = (sum_k A[i,k] * B[j,k]) * row_scale[i] * col_scale[j] + bias[j]
+ * A : i8[M,K], B : i8[N,K], scales and bias f32 (bias may be NULL), C : bf16[M,N] or f32[M,N].
+ * int32 sums, which are exact: K <= 131071 (EXO_B200_ERR_UNSUPPORTED above); scaled in fp32. */
+void gemm_i8_scaled_bf16_exo( void *ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const int8_t* A, const int8_t* B, const float* row_scale, const float* col_scale, const float* bias, uint16_t* C );
+void gemm_i8_scaled_f32_exo( void *ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const int8_t* A, const int8_t* B, const float* row_scale, const float* col_scale, const float* bias, float* C );
+
+/* linear_i8_*_exo: quantize_rows of X : [M,K] into Q : i8[M,K] and row_scale : f32[M] (both written),
+ * then gemm_i8_scaled of those with B.  Same results as the two calls. */
+void linear_i8_bf16_exo( void *ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const uint16_t* X, const int8_t* B, const float* col_scale, const float* bias, int8_t* Q, float* row_scale, uint16_t* Y );
+void linear_i8_f32_exo( void *ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const float* X, const int8_t* B, const float* col_scale, const float* bias, int8_t* Q, float* row_scale, float* Y );
+
+/* Activations of the gated projections: g / (1 + exp(-g)); g Phi(g); and Phi's tanh approximation
+ * g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))). */
+enum { EXO_B200_ACT_SILU = 0, EXO_B200_ACT_GELU = 1, EXO_B200_ACT_GELU_TANH = 2 };
+
+/* gated_bf16_exo: H = act(G) * U with G = X Wg^T, U = X Wu^T in one kernel (fp32 sums; H is formed from
+ * them before they are rounded).  X : bf16[M,K], Wg, Wu : bf16[F,K], H : bf16[M,F].  G and U : bf16[M,F]
+ * are written when they are not NULL (both or neither): what the backward pass needs. */
+void gated_bf16_exo( void *ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K, const uint16_t* X, const uint16_t* Wg, const uint16_t* Wu, uint16_t* H, uint16_t* G, uint16_t* U );
+
+/* gated_bf16_backward_exo: from the gradient dH : bf16[M,F] of gated_bf16_exo's H and its kept G, U:
+ *   dG = dH * U * act'(G), dU = dH * act(G)                     (written, bf16[M,F])
+ *   dX = dG Wg + dU Wu : bf16[M,K];  dWg = dG^T X, dWu = dU^T X : bf16[F,K]
+ * dX may be NULL (not computed), and so may dWg and dWu together.  The products take dG and dU as rounded
+ * to bf16; their sums are fp32 and rounded once. */
+void gated_bf16_backward_exo( void *ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K, const uint16_t* X, const uint16_t* Wg, const uint16_t* Wu, const uint16_t* G, const uint16_t* U, const uint16_t* dH, uint16_t* dG, uint16_t* dU, uint16_t* dX, uint16_t* dWg, uint16_t* dWu );
+
+/* gated_i8_bf16_exo: gated_bf16_exo on quantised operands: G = (A Bg^T) * row_scale * gate_scale,
+ * U = (A Bu^T) * row_scale * up_scale, H = act(G) * U : bf16[M,F].  A : i8[M,K], Bg, Bu : i8[F,K],
+ * row_scale : f32[M], gate_scale, up_scale : f32[F].  K <= 131071. */
+void gated_i8_bf16_exo( void *ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K, const int8_t* A, const int8_t* Bg, const int8_t* Bu, const float* row_scale, const float* gate_scale, const float* up_scale, uint16_t* H );
+
+/* ------------------------------------------------------------------------
  * Context and error side channel (additions; the reference has neither)
  * --------------------------------------------------------------------- */
 
