@@ -384,6 +384,7 @@ void exo_b200_context_destroy(exo_b200_Context* c) {
     if (c->scratch[i]) cudaFree(c->scratch[i]);
     if (c->scratch_ev[i]) cudaEventDestroy(c->scratch_ev[i]);
   }
+  if (c->pool) cudaMemPoolDestroy(c->pool);
   if (c->status_host) cudaFreeHost(c->status_host);
   if (c->pipe_ready) {
     cudaStreamDestroy(c->pipe_in);

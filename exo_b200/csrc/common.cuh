@@ -53,6 +53,7 @@ struct exo_b200_Context {
   cudaEvent_t scratch_ev[3];
   cudaStream_t scratch_stream[3];
   bool scratch_busy[3];
+  cudaMemPool_t pool;  // stream-ordered memory of single calls (operand copies of the feed-forward products)
   // weight cache (off unless exo_b200_context_cache_weights switched it on)
   bool cache_weights, wkey_valid;
   exob200::WeightKey wkey;

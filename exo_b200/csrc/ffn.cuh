@@ -27,10 +27,12 @@ struct Problem {
   int act;
 };
 
-// Both are ordered on the context's stream.
+// All are ordered on the context's stream.
 cudaError_t launch_quantize_rows(exo_b200_Context* ctx, int64_t M, int64_t K, const void* X, bool bf16, int8_t* Q,
                                  float* scale);
-cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p);
+// after_own_kernel: the kernel before this one on the stream belongs to the same call and was launched in the ordinary
+// way (or waits for one that was), so this one may be scheduled before it ends.
+cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p, bool after_own_kernel);
 // dG = dH * U * act'(G), dU = dH * act(G), n elements
 cudaError_t launch_gate_backward(exo_b200_Context* ctx, int act, int64_t n, const uint16_t* G, const uint16_t* U,
                                  const uint16_t* dH, uint16_t* dG, uint16_t* dU);

@@ -158,7 +158,7 @@ void gemm_scaled(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t N, int
   p.a0 = o.dev<void>(0), p.b0 = o.dev<void>(1);
   p.row_scale = o.dev<float>(2), p.col_scale = o.dev<float>(3), p.bias = o.dev<float>(4);
   p.c0 = o.dev<void>(5);
-  o.done(ffn::launch_product(o.ctx(), ffn::SCALED, f32, p));
+  o.done(ffn::launch_product(o.ctx(), ffn::SCALED, f32, p, false));
 }
 
 void linear(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const void* X,
@@ -185,7 +185,7 @@ void linear(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t N, int_fast
     p.a0 = o.dev<void>(4), p.b0 = o.dev<void>(1);
     p.row_scale = o.dev<float>(5), p.col_scale = o.dev<float>(2), p.bias = o.dev<float>(3);
     p.c0 = o.dev<void>(6);
-    err = ffn::launch_product(o.ctx(), ffn::SCALED, f32, p);
+    err = ffn::launch_product(o.ctx(), ffn::SCALED, f32, p, true);
   }
   o.done(err);
 }
@@ -241,7 +241,7 @@ void gated_bf16_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fas
   p.a0 = o.dev<void>(0), p.b0 = o.dev<void>(1), p.b1 = o.dev<void>(2);
   p.c0 = o.dev<void>(3), p.c1 = o.dev<void>(4), p.c2 = o.dev<void>(5);
   p.act = (int)activation;
-  o.done(ffn::launch_product(o.ctx(), ffn::GATED, false, p));
+  o.done(ffn::launch_product(o.ctx(), ffn::GATED, false, p, false));
 }
 
 void gated_bf16_backward_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
@@ -273,14 +273,14 @@ void gated_bf16_backward_exo(void* ctxt, int_fast32_t activation, int_fast32_t M
     p.M = M, p.N = K, p.K = F;
     p.a0 = o.dev<void>(6), p.a1 = o.dev<void>(7), p.b0 = o.dev<void>(1), p.b1 = o.dev<void>(2);
     p.c0 = o.dev<void>(8);
-    e = ffn::launch_product(o.ctx(), ffn::DGRAD, false, p);
+    e = ffn::launch_product(o.ctx(), ffn::DGRAD, false, p, true);
   }
   if (e == cudaSuccess && dWg) {
     ffn::Problem p{};
     p.M = F, p.N = K, p.K = M;
     p.a0 = o.dev<void>(6), p.a1 = o.dev<void>(7), p.b0 = o.dev<void>(0);
     p.c0 = o.dev<void>(9), p.c1 = o.dev<void>(10);
-    e = ffn::launch_product(o.ctx(), ffn::WGRAD, false, p);
+    e = ffn::launch_product(o.ctx(), ffn::WGRAD, false, p, true);
   }
   o.done(e);
 }
@@ -308,7 +308,7 @@ void gated_i8_bf16_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_
   p.row_scale = o.dev<float>(3), p.col_scale = o.dev<float>(4), p.col_scale1 = o.dev<float>(5);
   p.c0 = o.dev<void>(6);
   p.act = (int)activation;
-  o.done(ffn::launch_product(o.ctx(), ffn::GATED_I8, false, p));
+  o.done(ffn::launch_product(o.ctx(), ffn::GATED_I8, false, p, false));
 }
 
 }  // extern "C"

@@ -1,0 +1,573 @@
+// Feed-forward products on the tensor cores.
+//
+// split_kernel: one 128 x 128 accumulator per CTA (gated: 64 columns of the gate and the same 64 of the up projection
+// side by side, so that one thread of the epilogue meets both).  TMA -> mbarrier ring -> tcgen05.mma -> tensor memory,
+// as in tc_gemm.cu; the reduction is split over the CTAs of a cluster, which add their accumulators through
+// distributed shared memory in a fixed order, so results do not depend on timing.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "ffn.cuh"
+#include "tc_common.cuh"
+#include "umma.cuh"
+#include "umma_pair.cuh"
+
+namespace exob200 {
+namespace ffn {
+namespace {
+
+using namespace tc;
+using namespace umma;
+
+template <int KIND>
+struct Traits {
+  static constexpr bool I8 = KIND == SCALED || KIND == GATED_I8;
+  static constexpr bool TWO = KIND == GATED || KIND == GATED_I8;  // two weights, two accumulators side by side
+  static constexpr bool A_MN = KIND == WGRAD;                     // the reduction runs down A's rows
+  static constexpr bool B_MN = KIND == WGRAD || KIND == DGRAD;
+  static constexpr int ELEM = I8 ? 1 : 2;
+  static constexpr int BK = ROW_BYTES / ELEM;  // reduction elements of a stage
+  static constexpr int MMA = I8 ? KIND_I8 : KIND_F16;
+  __host__ __device__ static constexpr uint32_t idesc(uint32_t m, uint32_t n) {
+    return make_idesc(I8 ? 2 : 1, 1, 1, m, n) | (A_MN ? 1u << 15 : 0u) | (B_MN ? IDESC_B_MN_MAJOR : 0u);
+  }
+  // descriptor step of one MMA (32 bytes of the reduction) in units of 16 bytes
+  __host__ __device__ static constexpr uint64_t step(bool mn) { return mn ? (uint64_t)((32 / ELEM) * ROW_BYTES / 16) : 2u; }
+};
+
+struct Args {
+  int M, N;              // an output's rows and columns
+  int nkb, segments;     // k-blocks of one operand pair; DGRAD runs over two
+  int tiles_m, tiles_n;
+  int a_rows;            // rows of A's box (fewer than 128 when M is)
+  int vec;               // outputs take vector stores
+  int b_early;           // B and the scales of its columns are not written by the kernel before this one
+  const float *row_scale, *col_scale, *col_scale1, *bias;
+  void *c0, *c1, *c2;
+  DeviceStatus* status;
+};
+
+// ------------------------------------------------------------------ epilogue arithmetic
+template <class O>
+__device__ __forceinline__ void store4(O* p, const float (&v)[4], int left, bool vec);
+template <>
+__device__ __forceinline__ void store4<float>(float* p, const float (&v)[4], int left, bool vec) {
+  if (vec && left >= 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (j < left) p[j] = v[j];
+  }
+}
+template <>
+__device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, const float (&v)[4], int left, bool vec) {
+  if (vec && left >= 4) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (j < left) p[j] = __float2bfloat16_rn(v[j]);
+  }
+}
+
+// Four neighbouring columns of one output row, from finished sums.
+template <int KIND, class O, int ACT>
+__device__ __forceinline__ void finish4(const Args& p, int z, int row, int col, const uint32_t (&x)[4],
+                                        const uint32_t (&y)[4]) {
+  using T = Traits<KIND>;
+  const int left = p.N - col;
+  if (left <= 0) return;
+  const int64_t at = (int64_t)row * p.N + col;
+  float v[4], g[4], u[4];
+  if constexpr (T::I8) {
+    const float rs = p.row_scale[row];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int c = col + (j < left ? j : 0);
+      if constexpr (T::TWO) {
+        g[j] = scaled((int32_t)x[j], rs, __ldg(p.col_scale + c));
+        u[j] = scaled((int32_t)y[j], rs, __ldg(p.col_scale1 + c));
+      } else {
+        v[j] = scaled((int32_t)x[j], rs, __ldg(p.col_scale + c)) + (p.bias ? __ldg(p.bias + c) : 0.f);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      v[j] = g[j] = __uint_as_float(x[j]);
+      if constexpr (T::TWO) u[j] = __uint_as_float(y[j]);
+    }
+  }
+  if constexpr (T::TWO) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = gate<ACT>(g[j]) * u[j];
+    if (p.c1) {
+      store4(static_cast<O*>(p.c1) + at, g, left, p.vec);
+      store4(static_cast<O*>(p.c2) + at, u, left, p.vec);
+    }
+  }
+  store4(static_cast<O*>(KIND == WGRAD && z ? p.c1 : p.c0) + at, v, left, p.vec);
+}
+
+// ------------------------------------------------------------------ split kernel
+constexpr int S_STAGES = 3;                        // two CTAs share an SM: 2 x 3 x 32 KiB
+constexpr int S_STAGE_BYTES = 2 * A_TILE_BYTES;    // 128 rows of A, 128 of B
+constexpr int S_SMEM = S_STAGES * S_STAGE_BYTES + 1024 + 128;
+constexpr int S_PITCH = 132;                       // words between rows of the accumulator in shared memory: 128-bit
+                                                   // accesses of neighbouring rows fall on different banks
+static_assert(BM * S_PITCH * 4 <= S_STAGES * S_STAGE_BYTES, "the accumulator takes the ring's place");
+constexpr uint32_t S_TMEM_COLS = 128;
+constexpr int MAX_SPLIT = 8;
+
+__device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+template <bool I8>
+__device__ __forceinline__ uint32_t plus(uint32_t a, uint32_t b) {
+  return I8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+}
+// Sum over the cluster's CTAs of the four accumulator words at `offset`, always in the order of the ranks.
+template <bool I8, int S>
+__device__ __forceinline__ void cluster_sum(uint32_t base, uint32_t offset, uint32_t (&x)[4]) {
+  uint4 v[S];
+#pragma unroll
+  for (int s = 0; s < S; s++) v[s] = ld_cluster_v4(mapa(base, s) + offset);
+  x[0] = v[0].x, x[1] = v[0].y, x[2] = v[0].z, x[3] = v[0].w;
+#pragma unroll
+  for (int s = 1; s < S; s++) {
+    x[0] = plus<I8>(x[0], v[s].x);
+    x[1] = plus<I8>(x[1], v[s].y);
+    x[2] = plus<I8>(x[2], v[s].z);
+    x[3] = plus<I8>(x[3], v[s].w);
+  }
+}
+
+// Rows rank, rank + S, ... of the tile: sums over the cluster, epilogue, stores; a warp covers neighbouring columns.
+template <int KIND, class O, int ACT, int S>
+__device__ __forceinline__ void split_epilogue(const Args& p, uint32_t base, int rank, int z, int m0, int n0) {
+  using T = Traits<KIND>;
+  constexpr int GROUPS = T::TWO ? 16 : 32;  // groups of four output columns
+  const int rows = (min(BM, p.M - m0) - rank + S - 1) / S;
+  for (int i = threadIdx.x; i < rows * GROUPS; i += NUM_THREADS) {
+    const int r = rank + i / GROUPS * S, c = i % GROUPS * 4;
+    const uint32_t at = (uint32_t)(r * S_PITCH + c) * 4u;
+    uint32_t x[4], y[4] = {};
+    cluster_sum<T::I8, S>(base, at, x);
+    if constexpr (T::TWO) cluster_sum<T::I8, S>(base, at + 64 * 4, y);
+    finish4<KIND, O, ACT>(p, z, m0 + r, n0 + c, x, y);
+  }
+}
+
+template <int KIND, class O, int ACT>
+__global__ void __launch_bounds__(NUM_THREADS, 2)
+split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
+             const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+             const __grid_constant__ Args p, int S) {
+  using T = Traits<KIND>;
+  constexpr int BK = T::BK;
+  constexpr int CN = T::TWO ? 64 : 128;  // output columns of a tile
+  constexpr uint32_t IDESC = T::idesc(BM, 128);
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t tiles = (raw + 1023u) & ~1023u;
+  const uint32_t bars = tiles + S_STAGES * S_STAGE_BYTES;
+  uint8_t* ctrl = smem_raw + (bars - raw);
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (S_STAGES + s); };
+  const uint32_t done_bar = bars + 8u * (2 * S_STAGES);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl + 8 * (2 * S_STAGES + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * S_STAGES + 1) + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)blockIdx.x % S;  // the cluster is S consecutive CTAs
+  int t = (int)blockIdx.x / S;
+  const int per_z = p.tiles_m * p.tiles_n;
+  const int z = t / per_z;
+  t -= z * per_z;
+  const int m0 = t % p.tiles_m * BM, n0 = t / p.tiles_m * CN;
+  const int total = p.nkb * p.segments;
+  const int kb0 = (int)((int64_t)total * rank / S), n_kb = (int)((int64_t)total * (rank + 1) / S) - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S_STAGES; s++) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), S_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t a_bytes = T::A_MN ? (uint32_t)A_TILE_BYTES : (uint32_t)p.a_rows * ROW_BYTES;
+      auto load_a = [&](int s, int kb) {
+        const bool second = kb >= p.nkb;
+        const int k0 = (second ? kb - p.nkb : kb) * BK;
+        const CUtensorMap* m = second || (KIND == WGRAD && z) ? &tmA1 : &tmA0;
+        const uint32_t dst = tiles + s * S_STAGE_BYTES;
+        if (T::A_MN) {
+          for (int c = 0; c < 2; c++) tma_load_2d(dst + c * (A_TILE_BYTES / 2), m, full_bar(s), m0 + 64 * c, k0);
+        } else {
+          tma_load_2d(dst, m, full_bar(s), k0, m0);
+        }
+      };
+      auto load_b = [&](int s, int kb) {
+        const bool second = kb >= p.nkb;
+        const int k0 = (second ? kb - p.nkb : kb) * BK;
+        const uint32_t dst = tiles + s * S_STAGE_BYTES + A_TILE_BYTES;
+        if (T::TWO) {
+          tma_load_2d(dst, &tmB0, full_bar(s), k0, n0);
+          tma_load_2d(dst + A_TILE_BYTES / 2, &tmB1, full_bar(s), k0, n0);
+        } else if (T::B_MN) {
+          const CUtensorMap* m = second ? &tmB1 : &tmB0;
+          for (int c = 0; c < 2; c++) tma_load_2d(dst + c * (A_TILE_BYTES / 2), m, full_bar(s), n0 + 64 * c, k0);
+        } else {
+          tma_load_2d(dst, &tmB0, full_bar(s), k0, n0);
+        }
+      };
+      // The ring's first fill: what the kernel before this one does not write comes before waiting for that kernel.
+      const int first = min(n_kb, S_STAGES);
+      for (int i = 0; i < first; i++) mbar_arrive_expect_tx(full_bar(i), a_bytes + A_TILE_BYTES);
+      if (!p.b_early) grid_dep_wait();
+      for (int i = 0; i < first; i++) load_b(i, kb0 + i);
+      if (p.b_early) grid_dep_wait();
+      for (int i = 0; i < first; i++) load_a(i, kb0 + i);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = first; i < n_kb; i++) {
+        if (!mbar_wait(empty_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
+          report_timeout(p.status, abort_flag, 61);
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(full_bar(stage), a_bytes + A_TILE_BYTES);
+        load_b(stage, kb0 + i);
+        load_a(stage, kb0 + i);
+        if (++stage == S_STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok || *abort_flag) {  // error path: copies in flight land before the CTA leaves
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = 0; i < n_kb; i++) {
+        if (!mbar_wait(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
+          report_timeout(p.status, abort_flag, 62);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a0 = tiles + stage * S_STAGE_BYTES, b0 = a0 + A_TILE_BYTES;
+        const uint64_t da = T::A_MN ? smem_desc_mn_sw128(a0, BK) : smem_desc_k_sw128(a0);
+        const uint64_t db = T::B_MN ? smem_desc_mn_sw128(b0, BK) : smem_desc_k_sw128(b0);
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ks++)
+          tc_mma<T::MMA>(tmem, da + ks * T::step(T::A_MN), db + ks * T::step(T::B_MN), IDESC, (i | ks) != 0);
+        tc_commit(empty_bar(stage));
+        if (++stage == S_STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (ok) tc_commit(done_bar);
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;  // a warp reads the 32 tensor-memory lanes of its quarter
+    const int row = q * 32 + lane;
+    grid_dep_wait();  // the row scales may be the preceding kernel's
+    if (mbar_wait_warp(done_bar, 0, abort_flag, WAIT_LIMIT_NS)) {
+      tc_fence_after();
+      // every MMA has read its operands: the ring's shared memory takes the accumulator
+#pragma unroll 1
+      for (int ch = 0; ch < 4; ch++) {
+        uint32_t r[32];
+        tmem_ld_32x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ch * 32), r);
+        tmem_ld_wait();
+        if (m0 + row < p.M) {
+          const uint32_t dst = tiles + (uint32_t)(row * S_PITCH + ch * 32) * 4u;
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * 16), "r"(r[4 * j]),
+                         "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
+                         : "memory");
+        }
+      }
+      tc_fence_before();
+    } else if (lane == 0) {
+      report_timeout(p.status, abort_flag, 63);
+    }
+  }
+  // warps 0 and 1 read what the preceding kernel wrote in the epilogue, too
+  if (warp < 2) grid_dep_wait();
+  if (S > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  if (S == 1)
+    split_epilogue<KIND, O, ACT, 1>(p, tiles, rank, z, m0, n0);
+  else if (S == 2)
+    split_epilogue<KIND, O, ACT, 2>(p, tiles, rank, z, m0, n0);
+  else if (S == 4)
+    split_epilogue<KIND, O, ACT, 4>(p, tiles, rank, z, m0, n0);
+  else
+    split_epilogue<KIND, O, ACT, 8>(p, tiles, rank, z, m0, n0);
+  if (S > 1) cluster_sync_all();  // shared memory stays until every CTA of the cluster has read it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S_TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ operand copies with a pitch that TMA takes
+// TMA reads rows whose pitch and base are multiples of 16 bytes.  Other operands are multiplied from copies with the
+// pitch rounded up; each thread assembles 16 bytes from the aligned words around them.
+struct PadJob {
+  const uint8_t* src;
+  uint8_t* dst;
+  int64_t rows, src_pitch, dst_pitch;
+};
+constexpr int kMaxPads = 4;
+struct PadJobs {
+  PadJob job[kMaxPads];
+};
+
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ PadJobs jobs) {
+  const PadJob& j = jobs.job[blockIdx.y];
+  const int64_t per_row = j.dst_pitch / 16, n = j.rows * per_row;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 16;
+    const uint8_t* s = j.src + r * j.src_pitch + c;
+    const int left = (int)min((int64_t)16, j.src_pitch - c);  // bytes of this row from here on
+    const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(s) & 3u);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(s - shift);
+    uint32_t x[5];
+#pragma unroll
+    for (int k = 0; k < 5; k++) x[k] = 4 * k < left + (int)shift ? __ldg(w + k) : 0u;  // words that hold a byte of it
+    uint32_t y[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) y[k] = __funnelshift_r(x[k], x[k + 1], 8 * shift);
+    *reinterpret_cast<uint4*>(j.dst + r * j.dst_pitch + c) = make_uint4(y[0], y[1], y[2], y[3]);
+  }
+}
+
+// Memory of one call, ordered on its stream: freed behind the call's kernels, and inside a graph when the call is
+// captured, so that neither other streams nor other graphs ever see it.
+class StreamMemory {
+ public:
+  StreamMemory(exo_b200_Context* ctx) : ctx_(ctx) {}
+  ~StreamMemory() {
+    if (p_) cudaFreeAsync(p_, ctx_->stream);
+  }
+  StreamMemory(const StreamMemory&) = delete;
+  StreamMemory& operator=(const StreamMemory&) = delete;
+  cudaError_t get(size_t bytes) {
+    if (!ctx_->pool) {
+      cudaMemPoolProps props = {};
+      props.allocType = cudaMemAllocationTypePinned;
+      props.location.type = cudaMemLocationTypeDevice;
+      props.location.id = ctx_->device;
+      cudaError_t e = cudaMemPoolCreate(&ctx_->pool, &props);
+      if (e != cudaSuccess) {
+        ctx_->pool = nullptr;
+        return e;
+      }
+      uint64_t keep = UINT64_MAX;  // freed blocks stay for the next call instead of going back at a synchronisation
+      cudaMemPoolSetAttribute(ctx_->pool, cudaMemPoolAttrReleaseThreshold, &keep);
+    }
+    cudaError_t e = cudaMallocFromPoolAsync(&p_, bytes, ctx_->pool, ctx_->stream);
+    if (e != cudaSuccess) p_ = nullptr;
+    return e;
+  }
+  uint8_t* data() const { return static_cast<uint8_t*>(p_); }
+
+ private:
+  exo_b200_Context* ctx_;
+  void* p_ = nullptr;
+};
+
+// One operand: rows of `width` elements.
+struct Matrix {
+  const void* base;
+  int64_t rows, width, pitch;  // pitch in bytes
+};
+
+// Copies the operands that TMA cannot read; `copied` says whether any was.
+cudaError_t make_readable(exo_b200_Context* ctx, StreamMemory& memory, int elem, Matrix* const* ops, int n,
+                          bool* copied) {
+  PadJobs jobs;
+  int count = 0;
+  size_t bytes = 0;
+  int64_t most = 0;
+  int which[kMaxPads];
+  for (int i = 0; i < n; i++) {
+    Matrix& m = *ops[i];
+    if (m.pitch % 16 == 0 && aligned16(m.base)) continue;
+    const int64_t pitch = (m.width * elem + 15) / 16 * 16;
+    jobs.job[count] = PadJob{static_cast<const uint8_t*>(m.base), nullptr, m.rows, m.width * elem, pitch};
+    which[count++] = i;
+    bytes += (size_t)(m.rows * pitch);
+    most = std::max(most, m.rows * pitch / 16);
+  }
+  *copied = count > 0;
+  if (!count) return cudaSuccess;
+  cudaError_t e = memory.get(bytes);
+  if (e != cudaSuccess) return e;
+  uint8_t* at = memory.data();
+  for (int c = 0; c < count; c++) {
+    jobs.job[c].dst = at;
+    ops[which[c]]->base = at;
+    ops[which[c]]->pitch = jobs.job[c].dst_pitch;
+    at += jobs.job[c].rows * jobs.job[c].dst_pitch;
+  }
+  const unsigned grid = (unsigned)std::min<int64_t>((most + 255) / 256, (int64_t)ctx->sm_count * 8);
+  pad_rows_kernel<<<dim3(grid, (unsigned)count), 256, 0, ctx->stream>>>(jobs);
+  return cudaGetLastError();
+}
+
+bool map_of(CUtensorMap* m, const Matrix& x, int elem, int box_rows) {
+  cuuint64_t dims[2] = {(cuuint64_t)x.width, (cuuint64_t)x.rows};
+  cuuint64_t strides[1] = {(cuuint64_t)x.pitch};
+  cuuint32_t box[2] = {(cuuint32_t)(ROW_BYTES / elem), (cuuint32_t)box_rows};
+  return make_tiled_map(m, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x.base,
+                        dims, strides, box);
+}
+
+template <int KIND, class O, int ACT>
+cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], const Args& a, int64_t tiles,
+                         bool after_own_kernel) {
+  auto* kernel = split_kernel<KIND, O, ACT>;
+  EXOB200_SMEM_ATTR_ONCE(kernel, S_SMEM, ctx->device);
+  const int total = a.nkb * a.segments;
+  // split the reduction while the CTAs fit the GPU at two to an SM and each keeps four k-blocks
+  int S = 1;
+  while (S < MAX_SPLIT && tiles * S * 2 <= 2 * ctx->sm_count && total / (2 * S) >= 4) S *= 2;
+  if (tiles * S > INT32_MAX) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * S));
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = S_SMEM;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (S > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)S;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    n++;
+  }
+  if (after_own_kernel) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    n++;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a, S);
+}
+
+template <int KIND, class O, int ACT>
+cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kernel) {
+  using T = Traits<KIND>;
+  constexpr int E = T::ELEM;
+  auto matrix = [](const void* base, int64_t rows, int64_t width) { return Matrix{base, rows, width, width * E}; };
+  Matrix a0 = T::A_MN ? matrix(p.a0, p.K, p.M) : matrix(p.a0, p.M, p.K), a1 = a0;
+  a1.base = p.a1;
+  Matrix b0 = T::B_MN ? matrix(p.b0, p.K, p.N) : matrix(p.b0, p.N, p.K), b1 = b0;
+  b1.base = p.b1;
+  constexpr bool USES_A1 = KIND == WGRAD || KIND == DGRAD, USES_B1 = T::TWO || KIND == DGRAD;
+  Matrix* ops[4];
+  int n = 0;
+  ops[n++] = &a0;
+  if (USES_A1) ops[n++] = &a1;
+  ops[n++] = &b0;
+  if (USES_B1) ops[n++] = &b1;
+  StreamMemory memory(ctx);
+  bool copied = false;
+  cudaError_t e = make_readable(ctx, memory, E, ops, n, &copied);
+  if (e != cudaSuccess) return e;
+
+  Args a{};
+  a.M = (int)p.M, a.N = (int)p.N;
+  a.nkb = (int)((p.K + T::BK - 1) / T::BK);
+  a.segments = KIND == DGRAD ? 2 : 1;
+  a.row_scale = p.row_scale, a.col_scale = p.col_scale, a.col_scale1 = p.col_scale1, a.bias = p.bias;
+  a.c0 = p.c0, a.c1 = p.c1, a.c2 = p.c2;
+  a.status = ctx->status_dev;
+  a.b_early = copied ? 0 : 1;
+  constexpr int CN = T::TWO ? 64 : 128;
+  a.tiles_m = (int)((p.M + BM - 1) / BM);
+  a.tiles_n = (int)((p.N + CN - 1) / CN);
+  a.a_rows = (int)std::min<int64_t>(BM, (p.M + 7) / 8 * 8);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p.c0) | reinterpret_cast<uintptr_t>(p.c1) |
+                         reinterpret_cast<uintptr_t>(p.c2);
+  a.vec = p.N % 4 == 0 && bits % (4 * sizeof(O)) == 0;
+  CUtensorMap maps[4];
+  if (!map_of(&maps[0], a0, E, T::A_MN ? T::BK : a.a_rows)) return cudaErrorUnknown;
+  maps[1] = maps[0];
+  if (USES_A1 && !map_of(&maps[1], a1, E, T::A_MN ? T::BK : a.a_rows)) return cudaErrorUnknown;
+  const int b_rows = T::B_MN ? T::BK : T::TWO ? 64 : 128;
+  if (!map_of(&maps[2], b0, E, b_rows)) return cudaErrorUnknown;
+  maps[3] = maps[2];
+  if (USES_B1 && !map_of(&maps[3], b1, E, b_rows)) return cudaErrorUnknown;
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * (KIND == WGRAD ? 2 : 1);
+  return launch_split<KIND, O, ACT>(ctx, maps, a, tiles, after_own_kernel || copied);
+}
+
+}  // namespace
+
+cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p, bool after_own_kernel) {
+  using bf16 = __nv_bfloat16;
+  const bool own = after_own_kernel;
+  switch (kind) {
+    case SCALED:
+      return out_f32 ? launch<SCALED, float, 0>(ctx, p, own) : launch<SCALED, bf16, 0>(ctx, p, own);
+    case GATED:
+      return p.act == 0   ? launch<GATED, bf16, 0>(ctx, p, own)
+             : p.act == 1 ? launch<GATED, bf16, 1>(ctx, p, own)
+                          : launch<GATED, bf16, 2>(ctx, p, own);
+    case GATED_I8:
+      return p.act == 0   ? launch<GATED_I8, bf16, 0>(ctx, p, own)
+             : p.act == 1 ? launch<GATED_I8, bf16, 1>(ctx, p, own)
+                          : launch<GATED_I8, bf16, 2>(ctx, p, own);
+    case DGRAD:
+      return launch<DGRAD, bf16, 0>(ctx, p, own);
+    default:
+      return launch<WGRAD, bf16, 0>(ctx, p, own);
+  }
+}
+
+}  // namespace ffn
+}  // namespace exob200
