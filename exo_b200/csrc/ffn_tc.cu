@@ -4,6 +4,10 @@
 // side by side, so that one thread of the epilogue meets both).  TMA -> mbarrier ring -> tcgen05.mma -> tensor memory,
 // as in tc_gemm.cu; the reduction is split over the CTAs of a cluster, which add their accumulators through
 // distributed shared memory in a fixed order, so results do not depend on timing.
+//
+// pair_kernel: 256 x 256 tiles on CTA pairs (cta_group::2), persistent, for problems with enough of them.  The pair's
+// B tile is half in each CTA's shared memory: for the gated kinds the even CTA loads 128 rows of the gate's weight and
+// the odd one the same 128 rows of the up projection's, and every accumulator row holds both.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -351,6 +355,334 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
   }
 }
 
+// ------------------------------------------------------------------ pair kernel
+constexpr int P_STAGES = 5;                       // six let the pairs drift apart in L2 (tc_gemm2.cu)
+constexpr int P_STAGE_BYTES = 2 * A_TILE_BYTES;   // per CTA: 128 rows of A, its half (128) of B's columns
+constexpr int P_EPI_WARPS = 8;                    // two for each tensor-memory lane quarter, half the columns each
+constexpr int P_THREADS = 32 * (2 + P_EPI_WARPS);
+constexpr int P_STAGING = 8192;                   // per epilogue warp: two buffers of 32 rows x 128 bytes
+constexpr int P_CTRL = P_STAGES * P_STAGE_BYTES + P_EPI_WARPS * P_STAGING;
+constexpr int P_SMEM = P_CTRL + 1024 + 256;
+static_assert(P_SMEM <= 232448, "exceeds the shared memory a CTA can opt in to");
+constexpr int PN = 256;                           // accumulator columns of a tile
+constexpr uint32_t P_TMEM_COLS = 512;             // two accumulators
+
+struct PairMaps {
+  CUtensorMap a0, a1, b0, b1, c0, c1, c2;
+};
+
+// A warp's 32 x 32 block of one output, lane = row, `w` the row's packed values (two bf16 or one fp32 a word).
+// With a map for C: whole rows go out through the copy engine, which clips at C's edges; shared memory is
+// swizzled so that the 128-bit writes meet no bank twice.  Without (a pitch or base that TMA cannot take): rows leave
+// one by one, lane = column.
+template <class O>
+struct BlockStore {
+  static constexpr int WORDS = sizeof(O) == 2 ? 16 : 32;
+  uint32_t area;  // this warp's staging
+  int lane, buf = 0;
+
+  __device__ __forceinline__ void put(const uint32_t (&w)[WORDS], const CUtensorMap* m, O* C, const Args& p, int row0,
+                                      int col) {
+    if (row0 >= p.M || col >= p.N) return;
+    if (p.vec) {
+      if (lane == 0) bulk_wait_read_1();  // the store that last used this buffer has read it
+      __syncwarp();
+      const uint32_t at = area + (uint32_t)buf * 4096u;
+#pragma unroll
+      for (int j = 0; j < WORDS / 4; j++) {
+        const int swizzled = sizeof(O) == 2 ? j ^ ((lane >> 1) & 3) : j ^ (lane & 7);
+        const uint32_t dst = at + (uint32_t)(lane * WORDS * 4 + swizzled * 16);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[4 * j]), "r"(w[4 * j + 1]),
+                     "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                     : "memory");
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(m, at, col, row0);
+        bulk_commit();
+      }
+      buf ^= 1;
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < WORDS; j++)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(area + (uint32_t)(lane * (WORDS + 1) + j) * 4u), "r"(w[j]) : "memory");
+      __syncwarp();
+      const int rows = min(32, p.M - row0);
+      if (col + lane < p.N) {
+        O* out = C + (int64_t)row0 * p.N + col + lane;
+        for (int r = 0; r < rows; r++, out += p.N) {
+          const uint32_t src = area + (uint32_t)(r * (WORDS + 1) * 4 + lane * (int)sizeof(O));
+          if constexpr (sizeof(O) == 2) {
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
+            *reinterpret_cast<uint16_t*>(out) = v;
+          } else {
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(src) : "memory");
+            *reinterpret_cast<uint32_t*>(out) = v;
+          }
+        }
+      }
+    }
+  }
+};
+template <class O, int W>
+__device__ __forceinline__ void pack(const float (&v)[32], uint32_t (&w)[W]) {
+  if constexpr (sizeof(O) == 2) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
+  }
+}
+
+template <int KIND, class O, int ACT>
+__global__ void __launch_bounds__(P_THREADS, 1)
+pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args p, int group_rows) {
+  using T = Traits<KIND>;
+  constexpr int BK = T::BK;
+  constexpr int CN = T::TWO ? 128 : 256;  // output columns of a tile
+  constexpr uint32_t IDESC = T::idesc(2 * BM, PN);
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t tiles = (raw + 1023u) & ~1023u;
+  const uint32_t bars = tiles + P_CTRL;
+  uint8_t* ctrl = smem_raw + (bars - raw);
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (P_STAGES + s); };
+  auto tfull_bar = [&](int b) { return bars + 8u * (2 * P_STAGES + b); };
+  auto tempty_bar = [&](int b) { return bars + 8u * (2 * P_STAGES + 2 + b); };
+  const uint32_t slot_addr = bars + 8u * (2 * P_STAGES + 4);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl + 8 * (2 * P_STAGES + 4));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * P_STAGES + 4) + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();  // 0: owns full[] and tempty[], issues the MMAs
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < P_STAGES; s++) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), 2 * P_EPI_WARPS);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 1) {
+    tmem_alloc2(smem_u32(const_cast<uint32_t*>(tmem_slot)), P_TMEM_COLS);
+    tmem_relinquish2();
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+
+  const int per_z = p.tiles_m * p.tiles_n;
+  const int num_tiles = per_z * (KIND == WGRAD ? 2 : 1);
+  const int total = p.nkb * p.segments;
+  auto tile_coord = [&](int t, int& z, int& tm, int& tn) {
+    z = t / per_z;
+    t -= z * per_z;
+    const int per_group = group_rows * p.tiles_n, group = t / per_group, first = group * group_rows;
+    const int rows = min(group_rows, p.tiles_m - first), in_group = t - group * per_group;
+    tm = first + in_group % rows;
+    tn = in_group / rows;
+  };
+  auto give_up = [&](int where) {
+    report_timeout(p.status, abort_flag, where);
+    st_cluster_u32(mapa(slot_addr + 4, rank ^ 1u), 1u);  // take the partner down too
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+        int z, tm, tn;
+        tile_coord(t, z, tm, tn);
+        const int m0 = tm * 2 * BM + (int)rank * BM;
+        const int n0 = tn * CN + (T::TWO ? 0 : (int)rank * 128);
+        for (int kb = 0; kb < total; kb++) {
+          if (!mbar_wait_relaxed(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS, 50)) {
+            give_up(71);
+            ok = false;
+            break;
+          }
+          const uint32_t bar0 = mapa(full_bar(stage), 0);
+          const uint32_t a_dst = tiles + stage * P_STAGE_BYTES, b_dst = a_dst + A_TILE_BYTES;
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * P_STAGE_BYTES);
+          const bool second = kb >= p.nkb;
+          const int k0 = (second ? kb - p.nkb : kb) * BK;
+          const CUtensorMap* ma = second || (KIND == WGRAD && z) ? &maps.a1 : &maps.a0;
+          if (T::A_MN) {
+            for (int c = 0; c < 2; c++) tma_load_2d_pair(a_dst + c * (A_TILE_BYTES / 2), ma, bar0, m0 + 64 * c, k0);
+          } else {
+            tma_load_2d_pair(a_dst, ma, bar0, k0, m0);
+          }
+          if (T::TWO) {
+            tma_load_2d_pair(b_dst, rank ? &maps.b1 : &maps.b0, bar0, k0, n0);
+          } else if (T::B_MN) {
+            const CUtensorMap* mb = second ? &maps.b1 : &maps.b0;
+            for (int c = 0; c < 2; c++) tma_load_2d_pair(b_dst + c * (A_TILE_BYTES / 2), mb, bar0, n0 + 64 * c, k0);
+          } else {
+            tma_load_2d_pair(b_dst, &maps.b0, bar0, k0, n0);
+          }
+          if (++stage == P_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok || *abort_flag) {  // error path: copies in flight land before the CTA leaves
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
+          give_up(72);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(acc * PN);
+        for (int kb = 0; kb < total; kb++) {
+          if (!mbar_wait(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
+            give_up(73);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = tiles + stage * P_STAGE_BYTES, b0 = a0 + A_TILE_BYTES;
+          const uint64_t da = T::A_MN ? smem_desc_mn_sw128(a0, BK) : smem_desc_k_sw128(a0);
+          const uint64_t db = T::B_MN ? smem_desc_mn_sw128(b0, BK) : smem_desc_k_sw128(b0);
+#pragma unroll
+          for (int ks = 0; ks < KSTEPS; ks++)
+            tc_mma_pair<T::MMA>(d, da + ks * T::step(T::A_MN), db + ks * T::step(T::B_MN), IDESC, (kb | ks) != 0);
+          tc_commit_pair(empty_bar(stage));
+          if (++stage == P_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair(tfull_bar(acc));
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    BlockStore<O> store{tiles + P_STAGES * P_STAGE_BYTES + (uint32_t)(warp - 2) * P_STAGING, lane};
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int t = pair; t < num_tiles; t += num_pairs) {
+      int z, tm, tn;
+      tile_coord(t, z, tm, tn);
+      const int row0 = tm * 2 * BM + (int)rank * BM + q * 32, row = row0 + lane;
+      const int c0 = tn * CN + part * (CN / 2);
+      float rs = 0.f;
+      if constexpr (T::I8)
+        if (row < p.M) rs = p.row_scale[row];
+      if (!mbar_wait_warp(tfull_bar(acc), acc_phase, abort_flag, WAIT_LIMIT_NS)) {
+        if (lane == 0) give_up(74);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * PN + part * (CN / 2));
+#pragma unroll 1
+      for (int ch = 0; ch < CN / 64; ch++) {
+        const int col = c0 + ch * 32;
+        uint32_t x[32], w[BlockStore<O>::WORDS];
+        float v[32];
+        tmem_ld_32x32(from + (uint32_t)(ch * 32), x);
+        if constexpr (T::TWO) {
+          uint32_t y[32];
+          float u[32];
+          tmem_ld_32x32(from + (uint32_t)(128 + ch * 32), y);
+          tmem_ld_wait();
+          if constexpr (T::I8) {
+            // a lane holds the scales of one column; each column's reach every row of the block by a shuffle
+            const float cg = col + lane < p.N ? __ldg(p.col_scale + col + lane) : 0.f;
+            const float cu = col + lane < p.N ? __ldg(p.col_scale1 + col + lane) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              v[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, cg, j));
+              u[j] = scaled((int32_t)y[j], rs, __shfl_sync(0xffffffffu, cu, j));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              v[j] = __uint_as_float(x[j]);
+              u[j] = __uint_as_float(y[j]);
+            }
+            if (p.c1) {
+              pack<O>(v, w);
+              store.put(w, &maps.c1, static_cast<O*>(p.c1), p, row0, col);
+              pack<O>(u, w);
+              store.put(w, &maps.c2, static_cast<O*>(p.c2), p, row0, col);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] = gate<ACT>(v[j]) * u[j];
+        } else {
+          tmem_ld_wait();
+          if constexpr (T::I8) {
+            const float cs = col + lane < p.N ? __ldg(p.col_scale + col + lane) : 0.f;
+            const float add = p.bias && col + lane < p.N ? __ldg(p.bias + col + lane) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+              v[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, cs, j)) + __shfl_sync(0xffffffffu, add, j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = __uint_as_float(x[j]);
+          }
+        }
+        pack<O>(v, w);
+        if (KIND == WGRAD && z)
+          store.put(w, &maps.c1, static_cast<O*>(p.c1), p, row0, col);
+        else
+          store.put(w, &maps.c0, static_cast<O*>(p.c0), p, row0, col);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa(tempty_bar(acc), 0));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+    if (lane == 0) bulk_wait_all();  // shared memory outlives the stores that read it
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc2(tmem, P_TMEM_COLS);
+  }
+}
+
 // ------------------------------------------------------------------ operand copies with a pitch that TMA takes
 // TMA reads rows whose pitch and base are multiples of 16 bytes.  Other operands are multiplied from copies with the
 // pitch rounded up; each thread assembles 16 bytes from the aligned words around them.
@@ -465,6 +797,17 @@ bool map_of(CUtensorMap* m, const Matrix& x, int elem, int box_rows) {
                         dims, strides, box);
 }
 
+// Which kernel: EXOB200_FFN_PAIR=0 / 1 forces the split / the pair kernel.  Up to 128 rows the weights' bytes are what
+// counts, and the split kernel's CTAs share them out more evenly (1 x 16384 x 4096 gated: 47 against 73 us); above,
+// a pair's 256 x 256 tiles move half the operand bytes per flop (8192^3: 345 against 526 us).
+bool pair_wanted(int64_t rows, int64_t tiles) {
+  static const int mode = [] {
+    const char* e = getenv("EXOB200_FFN_PAIR");
+    return e ? atoi(e) : -1;
+  }();
+  return mode >= 0 ? mode == 1 : rows > 128 && tiles >= 64;
+}
+
 template <int KIND, class O, int ACT>
 cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], const Args& a, int64_t tiles,
                          bool after_own_kernel) {
@@ -499,6 +842,49 @@ cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], co
 }
 
 template <int KIND, class O, int ACT>
+cudaError_t launch_pair(exo_b200_Context* ctx, const PairMaps& maps, const Args& a, int64_t tiles, bool after_own_kernel) {
+  auto* kernel = pair_kernel<KIND, O, ACT>;
+  EXOB200_SMEM_ATTR_ONCE(kernel, P_SMEM, ctx->device);
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(P_THREADS);
+  cfg.dynamicSmemBytes = P_SMEM;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // every instance takes a whole SM, so all of them fit as many pairs; asked once per context
+  int& max_pairs = ctx->max_ffn_pairs;
+  if (max_pairs == 0) {
+    cfg.gridDim = dim3(2 * ctx->sm_count);
+    int n = 0;
+    cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess) return e;
+    max_pairs = std::max(1, n);
+  }
+  cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, max_pairs));
+  if (after_own_kernel) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, maps, a, 8);
+}
+
+// Tensor map of a dense output for 32 x 32 blocks out of swizzled shared memory
+template <class O>
+bool output_map(CUtensorMap* m, void* base, int64_t rows, int64_t cols) {
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)cols * sizeof(O)};
+  cuuint32_t box[2] = {32, 32};
+  return make_tiled_map(m, sizeof(O) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
+                        base, dims, strides, box,
+                        sizeof(O) == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int KIND, class O, int ACT>
 cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kernel) {
   using T = Traits<KIND>;
   constexpr int E = T::ELEM;
@@ -527,12 +913,34 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   a.c0 = p.c0, a.c1 = p.c1, a.c2 = p.c2;
   a.status = ctx->status_dev;
   a.b_early = copied ? 0 : 1;
-  constexpr int CN = T::TWO ? 64 : 128;
-  a.tiles_m = (int)((p.M + BM - 1) / BM);
-  a.tiles_n = (int)((p.N + CN - 1) / CN);
-  a.a_rows = (int)std::min<int64_t>(BM, (p.M + 7) / 8 * 8);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p.c0) | reinterpret_cast<uintptr_t>(p.c1) |
                          reinterpret_cast<uintptr_t>(p.c2);
+  const int Z = KIND == WGRAD ? 2 : 1;
+  auto tiles_of = [&](int64_t rows, int64_t cols) {
+    a.tiles_m = (int)((p.M + rows - 1) / rows);
+    a.tiles_n = (int)((p.N + cols - 1) / cols);
+    return (int64_t)a.tiles_m * a.tiles_n * Z;
+  };
+  int64_t tiles = tiles_of(2 * BM, T::TWO ? 128 : 256);
+  if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+  if (pair_wanted(p.M, tiles)) {
+    a.vec = p.N * (int64_t)sizeof(O) % 16 == 0 && bits % 16 == 0;
+    PairMaps m;
+    if (!map_of(&m.a0, a0, E, T::A_MN ? T::BK : BM)) return cudaErrorUnknown;
+    m.a1 = m.a0;
+    if (USES_A1 && !map_of(&m.a1, a1, E, T::A_MN ? T::BK : BM)) return cudaErrorUnknown;
+    if (!map_of(&m.b0, b0, E, T::B_MN ? T::BK : 128)) return cudaErrorUnknown;
+    m.b1 = m.b0;
+    if (USES_B1 && !map_of(&m.b1, b1, E, T::B_MN ? T::BK : 128)) return cudaErrorUnknown;
+    m.c0 = m.c1 = m.c2 = m.a0;
+    if (a.vec && !(output_map<O>(&m.c0, p.c0, p.M, p.N) && (!p.c1 || output_map<O>(&m.c1, p.c1, p.M, p.N)) &&
+                   (!p.c2 || output_map<O>(&m.c2, p.c2, p.M, p.N))))
+      return cudaErrorUnknown;
+    return launch_pair<KIND, O, ACT>(ctx, m, a, tiles, after_own_kernel || copied);
+  }
+  tiles = tiles_of(BM, T::TWO ? 64 : 128);
+  if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+  a.a_rows = (int)std::min<int64_t>(BM, (p.M + 7) / 8 * 8);
   a.vec = p.N % 4 == 0 && bits % (4 * sizeof(O)) == 0;
   CUtensorMap maps[4];
   if (!map_of(&maps[0], a0, E, T::A_MN ? T::BK : a.a_rows)) return cudaErrorUnknown;
@@ -542,7 +950,6 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   if (!map_of(&maps[2], b0, E, b_rows)) return cudaErrorUnknown;
   maps[3] = maps[2];
   if (USES_B1 && !map_of(&maps[3], b1, E, b_rows)) return cudaErrorUnknown;
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * (KIND == WGRAD ? 2 : 1);
   return launch_split<KIND, O, ACT>(ctx, maps, a, tiles, after_own_kernel || copied);
 }
 
