@@ -43,16 +43,29 @@ cudaError_t launch_gate_backward(exo_b200_Context* ctx, int act, int64_t n, cons
 // division are good to a few units of 2^-22 here, far inside the bf16 rounding of every result.
 __device__ __forceinline__ float logistic(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
-constexpr float kRootHalf = 0.70710678f;      // sqrt(1 / 2)
 constexpr float kRoot2Pi = 0.79788456f;       // sqrt(2 / pi)
 constexpr float kTanhCubic = 0.044715f;
 // beyond this p is 0 or 1 in fp32 for the two GELUs; keeps the cubic and its derivative finite
 constexpr float kGeluClamp = 32.0f;
 
+// The normal distribution function by formula 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions
+// (erfc(x) = t (a1 + a2 t + ... + a5 t^4) exp(-x^2), t = 1 / (1 + 0.3275911 x), within 1.5e-7): absolutely as close
+// as 1 + erf can be in fp32, at a third of erfcf's instructions (1000 x 4096 x 512 gated, both outputs: 17.8 us with
+// erfcf, 13.7 with this).
+__device__ __forceinline__ float normal_cdf(float g) {
+  const float t = __fdividef(1.0f, 1.0f + (0.3275911f * 0.70710678f) * fabsf(g));
+  float y = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  y = fmaf(t, y, 0.5f * 1.421413741f);
+  y = fmaf(t, y, 0.5f * -0.284496736f);
+  y = fmaf(t, y, 0.5f * 0.254829592f);
+  y = y * t * __expf(-0.5f * g * g);
+  return g < 0.0f ? y : 1.0f - y;
+}
+
 template <int ACT>
 __device__ __forceinline__ float gate_p(float g) {
   if (ACT == EXO_B200_ACT_SILU) return logistic(g);
-  if (ACT == EXO_B200_ACT_GELU) return 0.5f * erfcf(-kRootHalf * g);
+  if (ACT == EXO_B200_ACT_GELU) return normal_cdf(g);
   const float c = fminf(fmaxf(g, -kGeluClamp), kGeluClamp);
   return logistic(2.0f * kRoot2Pi * (c + kTanhCubic * c * c * c));
 }

@@ -79,43 +79,49 @@ __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, const fl
   }
 }
 
-// Four neighbouring columns of one output row, from finished sums.
-template <int KIND, class O, int ACT>
-__device__ __forceinline__ void finish4(const Args& p, int z, int row, int col, const uint32_t (&x)[4],
-                                        const uint32_t (&y)[4]) {
+// What a thread needs of four neighbouring output columns for any number of rows.
+template <int KIND>
+struct Columns {
   using T = Traits<KIND>;
-  const int left = p.N - col;
-  if (left <= 0) return;
-  const int64_t at = (int64_t)row * p.N + col;
+  int col, left;
+  float scale[T::I8 ? 4 : 1], scale1[T::I8 && T::TWO ? 4 : 1], bias[KIND == SCALED ? 4 : 1];
+
+  __device__ __forceinline__ Columns(const Args& p, int c) : col(c), left(p.N - c) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const bool in = j < left;
+      if constexpr (T::I8) scale[j] = in ? __ldg(p.col_scale + col + j) : 0.f;
+      if constexpr (T::I8 && T::TWO) scale1[j] = in ? __ldg(p.col_scale1 + col + j) : 0.f;
+      if constexpr (KIND == SCALED) bias[j] = in && p.bias ? __ldg(p.bias + col + j) : 0.f;
+    }
+  }
+};
+
+// Those columns of one output row, from finished sums.
+template <int KIND, class O, int ACT>
+__device__ __forceinline__ void finish4(const Args& p, const Columns<KIND>& k, int z, int row, float rs,
+                                        const uint32_t (&x)[4], const uint32_t (&y)[4]) {
+  using T = Traits<KIND>;
+  const int64_t at = (int64_t)row * p.N + k.col;
   float v[4], g[4], u[4];
-  if constexpr (T::I8) {
-    const float rs = p.row_scale[row];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int c = col + (j < left ? j : 0);
-      if constexpr (T::TWO) {
-        g[j] = scaled((int32_t)x[j], rs, __ldg(p.col_scale + c));
-        u[j] = scaled((int32_t)y[j], rs, __ldg(p.col_scale1 + c));
-      } else {
-        v[j] = scaled((int32_t)x[j], rs, __ldg(p.col_scale + c)) + (p.bias ? __ldg(p.bias + c) : 0.f);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
+  for (int j = 0; j < 4; j++) {
+    if constexpr (KIND == SCALED) {
+      v[j] = scaled((int32_t)x[j], rs, k.scale[j]) + k.bias[j];
+    } else if constexpr (KIND == GATED_I8) {
+      g[j] = scaled((int32_t)x[j], rs, k.scale[j]);
+      u[j] = scaled((int32_t)y[j], rs, k.scale1[j]);
+    } else {
       v[j] = g[j] = __uint_as_float(x[j]);
-      if constexpr (T::TWO) u[j] = __uint_as_float(y[j]);
+      u[j] = __uint_as_float(y[j]);
     }
+    if constexpr (T::TWO) v[j] = gate<ACT>(g[j]) * u[j];
   }
-  if constexpr (T::TWO) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = gate<ACT>(g[j]) * u[j];
-    if (p.c1) {
-      store4(static_cast<O*>(p.c1) + at, g, left, p.vec);
-      store4(static_cast<O*>(p.c2) + at, u, left, p.vec);
-    }
+  if (T::TWO && p.c1) {
+    store4(static_cast<O*>(p.c1) + at, g, k.left, p.vec);
+    store4(static_cast<O*>(p.c2) + at, u, k.left, p.vec);
   }
-  store4(static_cast<O*>(KIND == WGRAD && z ? p.c1 : p.c0) + at, v, left, p.vec);
+  store4(static_cast<O*>(KIND == WGRAD && z ? p.c1 : p.c0) + at, v, k.left, p.vec);
 }
 
 // ------------------------------------------------------------------ split kernel
@@ -156,19 +162,33 @@ __device__ __forceinline__ void cluster_sum(uint32_t base, uint32_t offset, uint
   }
 }
 
-// Rows rank, rank + S, ... of the tile: sums over the cluster, epilogue, stores; a warp covers neighbouring columns.
+// Rows rank, rank + S, ... of the tile: sums over the cluster, epilogue, stores.  A thread keeps its four columns and
+// goes down the rows, several at a time so that their shared-memory round trips overlap.
 template <int KIND, class O, int ACT, int S>
 __device__ __forceinline__ void split_epilogue(const Args& p, uint32_t base, int rank, int z, int m0, int n0) {
   using T = Traits<KIND>;
-  constexpr int GROUPS = T::TWO ? 16 : 32;  // groups of four output columns
+  constexpr int GROUPS = T::TWO ? 16 : 32;        // groups of four output columns
+  constexpr int STEP = NUM_THREADS / GROUPS;      // rows that the CTA covers at a time
+  constexpr int BATCH = S > 2 ? 2 : 4;
+  const Columns<KIND> cols(p, n0 + (int)threadIdx.x % GROUPS * 4);
+  if (cols.left <= 0) return;
   const int rows = (min(BM, p.M - m0) - rank + S - 1) / S;
-  for (int i = threadIdx.x; i < rows * GROUPS; i += NUM_THREADS) {
-    const int r = rank + i / GROUPS * S, c = i % GROUPS * 4;
-    const uint32_t at = (uint32_t)(r * S_PITCH + c) * 4u;
-    uint32_t x[4], y[4] = {};
-    cluster_sum<T::I8, S>(base, at, x);
-    if constexpr (T::TWO) cluster_sum<T::I8, S>(base, at + 64 * 4, y);
-    finish4<KIND, O, ACT>(p, z, m0 + r, n0 + c, x, y);
+  const uint32_t c = (uint32_t)threadIdx.x % GROUPS * 16u;
+  for (int first = threadIdx.x / GROUPS; first < rows; first += STEP * BATCH) {
+    uint32_t x[BATCH][4], y[BATCH][4] = {};
+    float rs[BATCH] = {};
+#pragma unroll
+    for (int b = 0; b < BATCH; b++) {
+      const int r = rank + min(first + b * STEP, rows - 1) * S;
+      if constexpr (T::I8) rs[b] = p.row_scale[m0 + r];
+      const uint32_t at = (uint32_t)(r * S_PITCH) * 4u + c;
+      cluster_sum<T::I8, S>(base, at, x[b]);
+      if constexpr (T::TWO) cluster_sum<T::I8, S>(base, at + 64 * 4, y[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; b++)
+      if (first + b * STEP < rows)
+        finish4<KIND, O, ACT>(p, cols, z, m0 + rank + (first + b * STEP) * S, rs[b], x[b], y[b]);
   }
 }
 
