@@ -33,6 +33,14 @@ cudaError_t launch_quantize_rows(exo_b200_Context* ctx, int64_t M, int64_t K, co
 // after_own_kernel: the kernel before this one on the stream belongs to the same call and was launched in the ordinary
 // way (or waits for one that was), so this one may be scheduled before it ends.
 cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p, bool after_own_kernel);
+// The products of a few rows (ffn_gemv.cu): whether they are taken for a problem, and their launch.
+constexpr int kRowTokenBytes = 96 * 1024;  // tokens that a CTA keeps in shared memory
+bool rows_wanted(Kind kind, const Problem& p);
+cudaError_t launch_rows(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p, bool after_own_kernel);
+// The same with the quantisation of the tokens X (bf16, or fp32 where the output is) in the one kernel; p.a0 and
+// p.row_scale are written.
+bool linear_rows_wanted(const Problem& p, bool f32);
+cudaError_t launch_linear_rows(exo_b200_Context* ctx, bool f32, const Problem& p, const void* X);
 // dG = dH * U * act'(G), dU = dH * act(G), n elements
 cudaError_t launch_gate_backward(exo_b200_Context* ctx, int act, int64_t n, const uint16_t* G, const uint16_t* U,
                                  const uint16_t* dH, uint16_t* dG, uint16_t* dU);
@@ -84,6 +92,46 @@ __device__ __forceinline__ float gate_slope(float g, float p) {
 
 __device__ __forceinline__ float scaled(int32_t acc, float row, float col) {
   return __int2float_rn(acc) * row * col;
+}
+
+// ------------------------------------------------------------------ quantisation of a row
+// Magnitudes compare like their bit patterns, and a NaN's is above infinity's.
+__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(fabsf(x)); }
+
+struct Step {
+  float inverse, up;  // q = nearest integer to (x * up) * inverse
+  bool finite;
+  float scale;
+};
+__device__ __forceinline__ Step step_of(unsigned top) {
+  Step s;
+  s.finite = top < 0x7f800000u;
+  const float t = __uint_as_float(top);
+  // 127 / top leaves fp32's range below 2^-121: such a row goes through with its values and top times 2^100
+  s.up = t < 0x1p-100f ? 0x1p100f : 1.0f;
+  s.inverse = s.finite && top ? __fdiv_rn(127.0f, t * s.up) : 0.0f;
+  s.scale = s.finite ? __fdiv_rn(t, 127.0f) : __uint_as_float(0x7fffffffu);
+  return s;
+}
+// Adding 1.5 * 2^23 in the same rounding as the product leaves the nearest integer in the low bits.
+__device__ __forceinline__ uint32_t quantized(float x, const Step& s) {
+  return s.finite ? __float_as_uint(fmaf(x * s.up, s.inverse, 12582912.0f)) & 0xffu : 0u;
+}
+
+template <class E>
+__device__ __forceinline__ void widen(const uint4& v, float (&f)[16 / sizeof(E)]);
+template <>
+__device__ __forceinline__ void widen<float>(const uint4& v, float (&f)[4]) {
+  f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+}
+template <>
+__device__ __forceinline__ void widen<__nv_bfloat16>(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    f[2 * j] = __uint_as_float(w[j] << 16);
+    f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+  }
 }
 
 }  // namespace ffn

@@ -178,14 +178,17 @@ void linear(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t N, int_fast
            .out(Y, mul(M, N, e), e)
            .stage())
     return;
-  cudaError_t err = ffn::launch_quantize_rows(o.ctx(), M, K, o.dev<void>(0), !f32, o.dev<int8_t>(4), o.dev<float>(5));
-  if (err == cudaSuccess) {
-    ffn::Problem p{};
-    p.M = M, p.N = N, p.K = K;
-    p.a0 = o.dev<void>(4), p.b0 = o.dev<void>(1);
-    p.row_scale = o.dev<float>(5), p.col_scale = o.dev<float>(2), p.bias = o.dev<float>(3);
-    p.c0 = o.dev<void>(6);
-    err = ffn::launch_product(o.ctx(), ffn::SCALED, f32, p, true);
+  ffn::Problem p{};
+  p.M = M, p.N = N, p.K = K;
+  p.a0 = o.dev<void>(4), p.b0 = o.dev<void>(1);
+  p.row_scale = o.dev<float>(5), p.col_scale = o.dev<float>(2), p.bias = o.dev<float>(3);
+  p.c0 = o.dev<void>(6);
+  cudaError_t err;
+  if (ffn::linear_rows_wanted(p, f32)) {
+    err = ffn::launch_linear_rows(o.ctx(), f32, p, o.dev<void>(0));
+  } else {
+    err = ffn::launch_quantize_rows(o.ctx(), M, K, o.dev<void>(0), !f32, o.dev<int8_t>(4), o.dev<float>(5));
+    if (err == cudaSuccess) err = ffn::launch_product(o.ctx(), ffn::SCALED, f32, p, true);
   }
   o.done(err);
 }

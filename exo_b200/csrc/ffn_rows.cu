@@ -11,45 +11,6 @@ using tc::aligned16;
 using umma::grid_dep_launch;
 
 // ------------------------------------------------------------------ quantisation
-// Magnitudes compare like their bit patterns, and a NaN's is above infinity's.
-__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(fabsf(x)); }
-
-struct Step {
-  float inverse, up;  // q = nearest integer to (x * up) * inverse
-  bool finite;
-  float scale;
-};
-__device__ __forceinline__ Step step_of(unsigned top) {
-  Step s;
-  s.finite = top < 0x7f800000u;
-  const float t = __uint_as_float(top);
-  // 127 / top leaves fp32's range below 2^-121: such a row goes through with its values and top times 2^100
-  s.up = t < 0x1p-100f ? 0x1p100f : 1.0f;
-  s.inverse = s.finite && top ? __fdiv_rn(127.0f, t * s.up) : 0.0f;
-  s.scale = s.finite ? __fdiv_rn(t, 127.0f) : __uint_as_float(0x7fffffffu);
-  return s;
-}
-// Adding 1.5 * 2^23 in the same rounding as the product leaves the nearest integer in the low bits.
-__device__ __forceinline__ uint32_t quantized(float x, const Step& s) {
-  return s.finite ? __float_as_uint(fmaf(x * s.up, s.inverse, 12582912.0f)) & 0xffu : 0u;
-}
-
-template <class E>
-__device__ __forceinline__ void widen(const uint4& v, float (&f)[16 / sizeof(E)]);
-template <>
-__device__ __forceinline__ void widen<float>(const uint4& v, float (&f)[4]) {
-  f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
-}
-template <>
-__device__ __forceinline__ void widen<__nv_bfloat16>(const uint4& v, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    f[2 * j] = __uint_as_float(w[j] << 16);
-    f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-  }
-}
-
 // Largest of the magnitudes over the WARPS warps that share a row.
 template <int WARPS>
 __device__ __forceinline__ unsigned row_top(unsigned top) {

@@ -990,6 +990,7 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
 cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p, bool after_own_kernel) {
   using bf16 = __nv_bfloat16;
   const bool own = after_own_kernel;
+  if (rows_wanted(kind, p)) return launch_rows(ctx, kind, out_f32, p, own);
   switch (kind) {
     case SCALED:
       return out_f32 ? launch<SCALED, float, 0>(ctx, p, own) : launch<SCALED, bf16, 0>(ctx, p, own);
