@@ -15,12 +15,14 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libexo_b200.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
+CALL = os.path.join(HERE, "_call.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -78,7 +80,25 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    build_call(force)
     return LIB
+
+
+def build_call(force: bool = False) -> "str | None":
+    """The Python binding's fast path (csrc/call.cpp), a plain CPython module.  The package works without it, only
+    slower by a few microseconds a call, so an interpreter without its headers is no error."""
+    src = os.path.join(CSRC, "call.cpp")
+    headers = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(headers, "Python.h")):
+        return None
+    if force or _stale(CALL, [src]):
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I", headers,
+               src, "-o", CALL]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+            raise RuntimeError("g++ failed for call.cpp")
+    return CALL
 
 
 if __name__ == "__main__":

@@ -625,3 +625,58 @@ def test_streams_and_contexts(lib):
                     lib.gated_bf16_exo(c, 0, M, F, K, xi, wg, wu, o, None, None)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", SIZES)
+def test_wrapper_refuses_wrong_device_tensors(lib, name):
+    """The compiled path hands what it does not take to the Python path, which says what is wrong; errors of the entry
+    point itself come back through it."""
+    import torch
+
+    import exo_b200
+
+    sizes = SIZES[name]
+    types = {"uint16": torch.bfloat16, "int8": torch.int8, "float32": torch.float32}
+    ops = [torch.ones(o.shape, dtype=types[str(o.dtype)], device="cuda") for o in operands(name, sizes)]
+    for i, o in enumerate(ops):
+        wrong = [o.double(), torch.cat([o.flatten(), o.flatten()[:1]]), 3, "x"]
+        if o.dim() == 2:
+            wrong.append(torch.ones(o.shape[::-1], dtype=o.dtype, device="cuda").T)
+        for w in wrong:
+            with pytest.raises(ValueError):
+                getattr(lib, name)(None, *sizes, *ops[:i], w, *ops[i + 1:])
+    with pytest.raises(exo_b200.ExoB200Error) as e:
+        getattr(lib, name)(None, *sizes, None, *ops[1:])
+    assert e.value.code == exo_b200.ERR_INVALID_ARGUMENT
+    with pytest.raises((exo_b200.ExoB200Error, ValueError)):
+        getattr(lib, name)(None, *[0] * len(sizes), *ops)
+    with pytest.raises(TypeError):
+        getattr(lib, name)(None, *sizes, *ops[1:])
+    with pytest.raises(ValueError):
+        getattr(lib, name)(None, *sizes, *ops, stream=1)
+    getattr(lib, name)(None, *sizes, *ops)
+    getattr(lib, name)(None, *(np.int64(n) for n in sizes), *ops)  # through the Python path
+
+
+@pytest.mark.gpu
+def test_entry_points_of_both_wrappers_agree_on_the_stream(lib):
+    """A checked and an unchecked entry point called in turn on two streams: each enqueues on its caller's."""
+    import torch
+
+    n = 256
+    w = torch.nn.Parameter(torch.randn(n, n, device="cuda").bfloat16(), requires_grad=False)
+    x, h, y = (torch.randn(n, n, device="cuda").bfloat16() for _ in range(3))
+    want = {}
+    streams = [torch.cuda.Stream(), torch.cuda.current_stream(), torch.cuda.Stream()]
+    for rep in range(4):
+        for s in streams:
+            torch.cuda.synchronize()
+            with torch.cuda.stream(s):
+                h.zero_(), y.zero_()
+                lib.gated_bf16_exo(None, 0, n, n, n, x, w, w, h, None, None)
+                lib.gemm_bf16_exo(None, n, n, n, h, w.data, y)
+                got = y.float().sum()
+            s.synchronize()
+            want.setdefault("y", float(got))
+            assert float(got) == want["y"] != 0.0
