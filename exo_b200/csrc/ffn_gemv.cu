@@ -5,7 +5,8 @@
 // cluster to set up: a warp takes R weight rows, reads them 512 bytes at a time with 16-byte loads that bypass L1,
 // multiplies against the tokens in shared memory (dp4a, or packed fp32 FMAs of widened bf16), adds over its lanes with
 // shuffles, and, where a row is split over KS warps of the CTA, over those through shared memory in a fixed order.
-// Rows that are not whole 16-byte vectors are read word by word, each shifted into place, so that no copy is needed.
+// Rows that do not start on 16 bytes are read by the vectors around them and shifted into place between neighbouring
+// lanes, so that no copy is needed.
 #include <type_traits>
 
 #include "ffn.cuh"
@@ -40,6 +41,37 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
+}
+
+// v: the aligned vector that holds the first 16 - shift of this lane's 16 bytes, the next lane's the rest (all lanes of
+// the warp call this).  Leaves the lane's bytes in v, those from `left` on as zeros.
+__device__ __forceinline__ void into_place(uint4& v, uint32_t shift, int left) {
+  const uint32_t bits = 8 * (shift & 3u);
+  auto next = [](uint32_t w) { return __shfl_down_sync(0xffffffffu, w, 1); };
+  auto join = [bits](uint32_t lo, uint32_t hi) { return __funnelshift_r(lo, hi, bits); };
+  switch (shift >> 2) {  // the same for the whole warp
+    case 0:
+      v = make_uint4(join(v.x, v.y), join(v.y, v.z), join(v.z, v.w), join(v.w, next(v.x)));
+      break;
+    case 1: {
+      const uint32_t a = next(v.x), b = next(v.y);
+      v = make_uint4(join(v.y, v.z), join(v.z, v.w), join(v.w, a), join(a, b));
+      break;
+    }
+    case 2: {
+      const uint32_t a = next(v.x), b = next(v.y), c = next(v.z);
+      v = make_uint4(join(v.z, v.w), join(v.w, a), join(a, b), join(b, c));
+      break;
+    }
+    default: {
+      const uint32_t a = next(v.x), b = next(v.y), c = next(v.z), d = next(v.w);
+      v = make_uint4(join(v.w, a), join(a, b), join(b, c), join(c, d));
+    }
+  }
+  if (left < 16) {
+    auto keep = [](uint32_t w, int n) { return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u); };
+    v = make_uint4(keep(v.x, left), keep(v.y, left - 4), keep(v.z, left - 8), keep(v.w, left - 12));
+  }
 }
 
 // ---- multiply-accumulate of one 32-bit word of weights and tokens
@@ -181,7 +213,9 @@ __device__ __forceinline__ void quantize_tokens(const RowArgs& p, uint8_t* s, in
 // Pieces of each row in flight in a warp.
 template <bool I8, int MR, bool VEC>
 __host__ __device__ constexpr int batch() {
-  return VEC ? (!I8 && MR <= 2 ? 4 : 2) : (MR == 1 ? 4 : 2);
+  // measured: bf16 1 x 16384 x 4096 gated 43.5 us with four, 44.7 with two; int8 21.8 with two, 22.7 with four;
+  // unaligned rows want registers more than loads in flight (K = 4095: 55.3 us with one, 66.6 with two)
+  return !VEC ? 1 : !I8 && MR <= 2 ? 4 : 2;
 }
 
 // XT: what the tokens are quantised from (void: they come as the product takes them).
@@ -192,7 +226,8 @@ row_kernel(const __grid_constant__ RowArgs p) {
   constexpr int E = I8 ? 1 : 2;
   constexpr int V = R * MR;
   constexpr int COLS = TWO ? R / 2 : R;  // output columns of a group
-  constexpr int PIECE = VEC ? 512 : 128; // bytes of a row that a warp reads at a time
+  // bytes of a row that a warp takes at a time; unaligned rows give lane 31's vector to lane 30
+  constexpr int PIECE = VEC ? 512 : 496;
   constexpr int BATCH = batch<I8, MR, VEC>();
   extern __shared__ __align__(16) uint8_t tokens[];
   __shared__ uint32_t sums[2][WARPS][V];
@@ -219,70 +254,47 @@ row_kernel(const __grid_constant__ RowArgs p) {
     Acc<I8> acc[R][MR];
     if (group < groups) {
       const uint8_t* row[R];
+      uint32_t shift[R];  // bytes of the first 16-byte vector in front of the row
 #pragma unroll
       for (int r = 0; r < R; r++) {
         // rows past the last are read again in its place; their sums are not stored
         const int n = min(col0 + (TWO ? r % COLS : r), p.N - 1);
         row[r] = static_cast<const uint8_t*>(TWO && r >= COLS ? p.w1 : p.w0) + (int64_t)n * row_bytes;
+        shift[r] = VEC ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(row[r]) & 15u);
+        row[r] -= shift[r];
       }
       for (int piece = ks; piece < pieces; piece += p.k_split * BATCH) {
-        if constexpr (VEC) {
-          uint4 w[BATCH][R];
+        uint4 w[BATCH][R];
 #pragma unroll
-          for (int b = 0; b < BATCH; b++) {
-            const int at = (piece + b * p.k_split) * 512 + lane * 16;
+        for (int b = 0; b < BATCH; b++) {
+          const int at = (piece + b * p.k_split) * PIECE + lane * 16;
 #pragma unroll
-            for (int r = 0; r < R; r++) w[b][r] = at < row_bytes ? ld_stream(row[r] + at) : make_uint4(0, 0, 0, 0);
+          for (int r = 0; r < R; r++)  // vectors that hold a byte of the row
+            w[b][r] = at < row_bytes + (int)shift[r] ? ld_stream(row[r] + at) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+          const int at = (piece + b * p.k_split) * PIECE + lane * 16;
+          if (!VEC) {
+#pragma unroll
+            for (int r = 0; r < R; r++) into_place(w[b][r], shift[r], row_bytes - at);
+            if (lane == 31) continue;  // its vector was the other half of lane 30's
           }
+          if (at >= pitch) continue;
 #pragma unroll
-          for (int b = 0; b < BATCH; b++) {
-            const int at = (piece + b * p.k_split) * 512 + lane * 16;
-            if (at >= pitch) break;
-#pragma unroll
-            for (int m = 0; m < MR; m++) {
-              if (MR > 1 && m >= p.M) break;
-              const uint4 x = *reinterpret_cast<const uint4*>(tokens + m * pitch + at);
-              const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int r = 0; r < R; r++) {
-                const uint32_t ws[4] = {w[b][r].x, w[b][r].y, w[b][r].z, w[b][r].w};
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                  if constexpr (I8)
-                    acc[r][m].mac(ws[j], xs[j]);
-                  else
-                    acc[r][m].mac(widen_pair(ws[j]), widen_pair(xs[j]));
-                }
-              }
-            }
-          }
-        } else {
-#pragma unroll
-          for (int b = 0; b < BATCH; b++) {
-            const int at = (piece + b * p.k_split) * 128 + lane * 4;  // this lane's four bytes of the row
-            if (at >= row_bytes) break;
-            uint32_t w[R];
+          for (int m = 0; m < MR; m++) {
+            if (MR > 1 && m >= p.M) break;
+            const uint4 x = *reinterpret_cast<const uint4*>(tokens + m * pitch + at);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int r = 0; r < R; r++) {
-              // the two aligned words around them; the second only where it holds one of the row's bytes
-              const uint8_t* a = row[r] + at;
-              const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(a) & 3u);
-              const uint32_t* word = reinterpret_cast<const uint32_t*>(a - shift);
-              const int left = row_bytes - at;
-              const uint32_t lo = __ldg(word), hi = left + (int)shift > 4 ? __ldg(word + 1) : 0u;
-              w[r] = __funnelshift_r(lo, hi, 8 * shift);
-              if (left < 4) w[r] &= (1u << (8 * left)) - 1u;
-            }
+              const uint32_t ws[4] = {w[b][r].x, w[b][r].y, w[b][r].z, w[b][r].w};
 #pragma unroll
-            for (int m = 0; m < MR; m++) {
-              if (MR > 1 && m >= p.M) break;
-              const uint32_t x = *reinterpret_cast<const uint32_t*>(tokens + m * pitch + at);
-#pragma unroll
-              for (int r = 0; r < R; r++) {
+              for (int j = 0; j < 4; j++) {
                 if constexpr (I8)
-                  acc[r][m].mac(w[r], x);
+                  acc[r][m].mac(ws[j], xs[j]);
                 else
-                  acc[r][m].mac(widen_pair(w[r]), widen_pair(x));
+                  acc[r][m].mac(widen_pair(ws[j]), widen_pair(xs[j]));
               }
             }
           }
@@ -367,10 +379,10 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   }
   const bool vec = row_bytes % 16 == 0 && aligned16(p.b0) && (KIND == SCALED || aligned16(p.b1));
   const int64_t groups = (p.N + COLS - 1) / COLS;
-  // 16 warps an SM keep the memory busy: split rows over the CTA's warps while there are fewer than that
+  // eight warps an SM keep the memory busy: split rows over the CTA's warps while there are fewer than that
   a.k_split = 1;
-  const int64_t pieces = (row_bytes + (vec ? 511 : 127)) / (vec ? 512 : 128);
-  while (a.k_split < WARPS && groups * a.k_split < (vec ? 8 : 16) * ctx->sm_count && pieces >= 2 * a.k_split) a.k_split *= 2;
+  const int64_t piece = vec ? 512 : 496, pieces = (row_bytes + piece - 1) / piece;
+  while (a.k_split < WARPS && groups * a.k_split < 8 * ctx->sm_count && pieces >= 2 * a.k_split) a.k_split *= 2;
   const int64_t ctas = (groups * a.k_split + WARPS - 1) / WARPS;
   const size_t smem = (size_t)(p.M * ((row_bytes + 511) / 512 * 512));
   const int per_sm = smem <= 32768 ? 4 : 2;

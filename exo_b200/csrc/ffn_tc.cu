@@ -12,6 +12,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "ffn.cuh"
 #include "tc_common.cuh"
@@ -51,6 +52,8 @@ struct Args {
   const float *row_scale, *col_scale, *col_scale1, *bias;
   void *c0, *c1, *c2;
   DeviceStatus* status;
+  const uint8_t *a, *b, *b1;  // operands that are gathered instead of copied by TMA; rows of row_bytes
+  int row_bytes;
 };
 
 // ------------------------------------------------------------------ epilogue arithmetic
@@ -164,11 +167,11 @@ __device__ __forceinline__ void cluster_sum(uint32_t base, uint32_t offset, uint
 
 // Rows rank, rank + S, ... of the tile: sums over the cluster, epilogue, stores.  A thread keeps its four columns and
 // goes down the rows, several at a time so that their shared-memory round trips overlap.
-template <int KIND, class O, int ACT, int S>
+template <int KIND, class O, int ACT, int THREADS, int S>
 __device__ __forceinline__ void split_epilogue(const Args& p, uint32_t base, int rank, int z, int m0, int n0) {
   using T = Traits<KIND>;
   constexpr int GROUPS = T::TWO ? 16 : 32;        // groups of four output columns
-  constexpr int STEP = NUM_THREADS / GROUPS;      // rows that the CTA covers at a time
+  constexpr int STEP = THREADS / GROUPS;          // rows that the CTA covers at a time
   constexpr int BATCH = S > 2 ? 2 : 4;
   const Columns<KIND> cols(p, n0 + (int)threadIdx.x % GROUPS * 4);
   if (cols.left <= 0) return;
@@ -192,20 +195,153 @@ __device__ __forceinline__ void split_epilogue(const Args& p, uint32_t base, int
   }
 }
 
-template <int KIND, class O, int ACT>
-__global__ void __launch_bounds__(NUM_THREADS, 2)
+// ---- gathered operands
+// Rows whose pitch or base TMA cannot take are read by the aligned 16-byte vectors around them (nine for 128 bytes),
+// asynchronously into a ring of raw rows in shared memory, and shifted from there into the swizzled tile.  A warp
+// shifts what it has fetched itself, so no two warps wait for one another.
+constexpr int G_WARPS = 8;                      // warps 2 .. 9 gather
+constexpr int G_THREADS = 64 + 32 * G_WARPS;
+constexpr int G_STAGES = 2;                     // swizzled tiles
+constexpr int G_RAW_ROW = ROW_BYTES + 16;
+constexpr int G_MAX_M = 32;                     // tokens: with more, shifting takes longer than copies do
+constexpr int G_DEPTH = 3;                      // raw k-blocks, two of them in flight while one is shifted
+constexpr int G_A_TILE = G_MAX_M * ROW_BYTES, G_STAGE_BYTES = G_A_TILE + A_TILE_BYTES;
+constexpr int G_RAW = (G_MAX_M + BM) * G_RAW_ROW;
+constexpr int G_AREA = G_STAGES * G_STAGE_BYTES + G_DEPTH * G_RAW;
+constexpr int G_SMEM = G_AREA + 1024 + 128;
+static_assert(G_AREA >= BM * S_PITCH * 4, "the accumulator takes the rings' place");
+static_assert(2 * (G_SMEM + 1024) <= 233472, "two CTAs share an SM");
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
+  const int bytes = in ? 16 : 0;  // zeros otherwise
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// One row of an operand as eight lanes share it.
+struct GatherRow {
+  const uint8_t* aligned;  // the row's first vector; nullptr: no such row
+  uint32_t shift;          // bytes of it in front of the row
+
+  __device__ __forceinline__ void set(const uint8_t* row) {
+    shift = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15u);
+    aligned = row ? row - shift : nullptr;
+  }
+  // vectors [at, at + 144) of the row, those that hold none of its bytes as zeros
+  __device__ __forceinline__ void fetch(uint32_t raw, int at, int row_bytes, int v) const {
+    if (!aligned) return;
+    const int end = row_bytes + (int)shift;
+    cp_async16(raw + v * 16, at + v * 16 < end ? aligned + at + v * 16 : aligned, at + v * 16 < end);
+    if (v == 7) cp_async16(raw + 128, at + 128 < end ? aligned + at + 128 : aligned, at + 128 < end);
+  }
+  // bytes [at + 16 v, + 16) of the row to their swizzled place in line r of a tile
+  __device__ __forceinline__ void place(uint32_t raw, uint32_t tile, int r, int at, int row_bytes, int v) const {
+    if (!aligned) return;
+    const uint4 lo = ld_shared16(raw + v * 16), hi = ld_shared16(raw + v * 16 + 16);
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    const bool two = shift & 8u, one = shift & 4u;  // differs between the warp's rows: selects, no branches
+#pragma unroll
+    for (int j = 0; j < 6; j++) w[j] = two ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < 5; j++) w[j] = one ? w[j + 1] : w[j];
+    uint32_t y[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) y[j] = __funnelshift_r(w[j], w[j + 1], 8 * (shift & 3u));
+    const int left = row_bytes - at - v * 16;
+    if (left < 16) {  // nothing behind the row's end may reach a sum
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int keep = left - 4 * j;
+        if (keep < 4) y[j] = keep <= 0 ? 0u : y[j] & ((1u << (8 * keep)) - 1u);
+      }
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + (uint32_t)(r * ROW_BYTES + ((v ^ (r & 7)) * 16))),
+                 "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
+                 : "memory");
+  }
+};
+
+// The gathering warps' part of a CTA: warp w takes rows 4 (w + 8 i) + lane / 8 of the B tile and of A.
+template <int KIND>
+__device__ __forceinline__ void gather(const Args& p, uint32_t tiles, uint32_t full0, uint32_t empty0,
+                                       volatile int* abort_flag, int w, int lane, int m0, int n0, int kb0, int n_kb) {
+  using T = Traits<KIND>;
+  constexpr int B_ROWS = BM / (4 * G_WARPS);
+  const uint32_t raw0 = tiles + G_STAGES * G_STAGE_BYTES;
+  const int v = lane & 7, first = w * 4 + lane / 8;
+  GatherRow a, b[B_ROWS];
+  a.set(m0 + first < p.M ? p.a + (int64_t)(m0 + first) * p.row_bytes : nullptr);
+#pragma unroll
+  for (int i = 0; i < B_ROWS; i++) {
+    const int r = first + 32 * i, n = n0 + (T::TWO ? r % 64 : r);
+    b[i].set(n < p.N ? (T::TWO && r >= 64 ? p.b1 : p.b) + (int64_t)n * p.row_bytes : nullptr);
+  }
+  auto fetch = [&](int i) {
+    if (i < n_kb) {
+      const uint32_t raw = raw0 + (uint32_t)(i % G_DEPTH * G_RAW);
+      const int at = (kb0 + i) * ROW_BYTES;
+      a.fetch(raw + first * G_RAW_ROW, at, p.row_bytes, v);
+#pragma unroll
+      for (int j = 0; j < B_ROWS; j++)
+        b[j].fetch(raw + (G_MAX_M + first + 32 * j) * G_RAW_ROW, at, p.row_bytes, v);
+    }
+    cp_async_commit();  // a group for every k-block, empty ones behind the last
+  };
+#pragma unroll
+  for (int i = 0; i < G_DEPTH - 1; i++) fetch(i);
+  int stage = 0;
+  uint32_t phase = 1;
+  for (int i = 0; i < n_kb; i++) {
+    fetch(i + G_DEPTH - 1);  // into the slot that this warp has read in the last round
+    cp_async_wait<G_DEPTH - 1>();
+    // the lanes decide together, so that none is left alone at a barrier
+    if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8u * stage, phase, abort_flag, WAIT_LIMIT_NS))) {
+      if (lane == 0) report_timeout(p.status, abort_flag, 64);
+      break;
+    }
+    const uint32_t raw = raw0 + (uint32_t)(i % G_DEPTH * G_RAW), a_dst = tiles + stage * G_STAGE_BYTES;
+    const int at = (kb0 + i) * ROW_BYTES;
+    a.place(raw + first * G_RAW_ROW, a_dst, first, at, p.row_bytes, v);
+#pragma unroll
+    for (int j = 0; j < B_ROWS; j++)
+      b[j].place(raw + (G_MAX_M + first + 32 * j) * G_RAW_ROW, a_dst + G_A_TILE, first + 32 * j, at, p.row_bytes, v);
+    fence_proxy_async();  // the tensor core reads what was stored here
+    __syncwarp();
+    if (lane == 0) mbar_arrive(full0 + 8u * stage);
+    if (++stage == G_STAGES) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  cp_async_wait<0>();
+}
+
+template <int KIND, class O, int ACT, bool GATHER>
+__global__ void __launch_bounds__(GATHER ? G_THREADS : NUM_THREADS, 2)
 split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
              const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
              const __grid_constant__ Args p, int S) {
   using T = Traits<KIND>;
   constexpr int BK = T::BK;
   constexpr int CN = T::TWO ? 64 : 128;  // output columns of a tile
+  constexpr int THREADS = GATHER ? G_THREADS : NUM_THREADS;
   constexpr uint32_t IDESC = T::idesc(BM, 128);
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t tiles = (raw + 1023u) & ~1023u;
-  const uint32_t bars = tiles + S_STAGES * S_STAGE_BYTES;
+  constexpr int STAGES = GATHER ? G_STAGES : S_STAGES;
+  constexpr int A_TILE = GATHER ? G_A_TILE : A_TILE_BYTES, STAGE_BYTES = A_TILE + A_TILE_BYTES;
+  const uint32_t bars = tiles + (GATHER ? G_AREA : S_STAGES * S_STAGE_BYTES);
   uint8_t* ctrl = smem_raw + (bars - raw);
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (S_STAGES + s); };
@@ -225,7 +361,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S_STAGES; s++) {
-      mbar_init(full_bar(s), 1);
+      mbar_init(full_bar(s), GATHER ? G_WARPS : 1);
       mbar_init(empty_bar(s), 1);
     }
     mbar_init(done_bar, 1);
@@ -233,7 +369,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
     fence_barrier_init();
     fence_proxy_async();
   }
-  if (warp == 2 && lane == 0) {  // the descriptors' first fetch overlaps the set-up
+  if (!GATHER && warp == 2 && lane == 0) {  // the descriptors' first fetch overlaps the set-up
     prefetch_tensormap(&tmA0);
     prefetch_tensormap(&tmB0);
     if (KIND == WGRAD || KIND == DGRAD) prefetch_tensormap(&tmA1);
@@ -249,7 +385,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (!GATHER && lane == 0) {
       const uint32_t a_bytes = T::A_MN ? (uint32_t)A_TILE_BYTES : (uint32_t)p.a_rows * ROW_BYTES;
       auto load_a = [&](int s, int kb) {
         const bool second = kb >= p.nkb;
@@ -319,14 +455,14 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
           break;
         }
         tc_fence_after();
-        const uint32_t a0 = tiles + stage * S_STAGE_BYTES, b0 = a0 + A_TILE_BYTES;
+        const uint32_t a0 = tiles + stage * STAGE_BYTES, b0 = a0 + A_TILE;
         const uint64_t da = T::A_MN ? smem_desc_mn_sw128(a0, BK) : smem_desc_k_sw128(a0);
         const uint64_t db = T::B_MN ? smem_desc_mn_sw128(b0, BK) : smem_desc_k_sw128(b0);
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ks++)
           tc_mma<T::MMA>(tmem, da + ks * T::step(T::A_MN), db + ks * T::step(T::B_MN), IDESC, (i | ks) != 0);
         tc_commit(empty_bar(stage));
-        if (++stage == S_STAGES) {
+        if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
         }
@@ -338,7 +474,9 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
     const int q = warp & 3;  // a warp reads the 32 tensor-memory lanes of its quarter
     const int row = q * 32 + lane;
     grid_dep_wait();  // the row scales may be the preceding kernel's
-    if (mbar_wait_warp(done_bar, 0, abort_flag, WAIT_LIMIT_NS)) {
+    if constexpr (GATHER)
+      gather<KIND>(p, tiles, full_bar(0), empty_bar(0), abort_flag, warp - 2, lane, m0, n0, kb0, n_kb);
+    if (warp < 6 && mbar_wait_warp(done_bar, 0, abort_flag, WAIT_LIMIT_NS)) {
       tc_fence_after();
       // every MMA has read its operands: the ring's shared memory takes the accumulator
 #pragma unroll 1
@@ -356,7 +494,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
         }
       }
       tc_fence_before();
-    } else if (lane == 0) {
+    } else if (warp < 6 && lane == 0) {
       report_timeout(p.status, abort_flag, 63);
     }
   }
@@ -367,13 +505,13 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
   else
     __syncthreads();
   if (S == 1)
-    split_epilogue<KIND, O, ACT, 1>(p, tiles, rank, z, m0, n0);
+    split_epilogue<KIND, O, ACT, THREADS, 1>(p, tiles, rank, z, m0, n0);
   else if (S == 2)
-    split_epilogue<KIND, O, ACT, 2>(p, tiles, rank, z, m0, n0);
+    split_epilogue<KIND, O, ACT, THREADS, 2>(p, tiles, rank, z, m0, n0);
   else if (S == 4)
-    split_epilogue<KIND, O, ACT, 4>(p, tiles, rank, z, m0, n0);
+    split_epilogue<KIND, O, ACT, THREADS, 4>(p, tiles, rank, z, m0, n0);
   else
-    split_epilogue<KIND, O, ACT, 8>(p, tiles, rank, z, m0, n0);
+    split_epilogue<KIND, O, ACT, THREADS, 8>(p, tiles, rank, z, m0, n0);
   if (S > 1) cluster_sync_all();  // shared memory stays until every CTA of the cluster has read it
   if (warp == 1) {
     tc_fence_after();
@@ -840,20 +978,33 @@ bool pair_wanted(int64_t rows, int64_t tiles) {
   return mode >= 0 ? mode == 1 : rows > 128 && tiles >= 64;
 }
 
-template <int KIND, class O, int ACT>
+// Operands that TMA cannot read: gathered as they are, or copied first.  Measured, gathered / copied: 16 x 16384 x 4095
+// gated bf16 95 / 141 us, int8 51 / 72, 16 x 4099 x 4099 int8 15.1 / 15.9, small ones 1 to 2 us slower on the GPU but
+// 3 us less for the host, which has neither memory to order nor a second launch; with 64 tokens 174 / 142 us.
+// EXOB200_FFN_GATHER=0 switches it off.
+bool gather_wanted(int64_t rows) {
+  static const bool off = [] {
+    const char* e = getenv("EXOB200_FFN_GATHER");
+    return e && e[0] == '0';
+  }();
+  return !off && rows <= G_MAX_M;
+}
+
+template <int KIND, class O, int ACT, bool GATHER>
 cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], const Args& a, int64_t tiles,
                          bool after_own_kernel) {
-  auto* kernel = split_kernel<KIND, O, ACT>;
-  EXOB200_SMEM_ATTR_ONCE(kernel, S_SMEM, ctx->device);
+  auto* kernel = split_kernel<KIND, O, ACT, GATHER>;
+  constexpr int SMEM = GATHER ? G_SMEM : S_SMEM;
+  EXOB200_SMEM_ATTR_ONCE(kernel, SMEM, ctx->device);
   const int total = a.nkb * a.segments;
-  // split the reduction while the CTAs fit the GPU at two to an SM and each keeps four k-blocks
+  // split the reduction while the CTAs fit the GPU at once and each keeps four k-blocks
   int S = 1;
   while (S < MAX_SPLIT && tiles * S * 2 <= 2 * ctx->sm_count && total / (2 * S) >= 4) S *= 2;
   if (tiles * S > INT32_MAX) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * S));
-  cfg.blockDim = dim3(NUM_THREADS);
-  cfg.dynamicSmemBytes = S_SMEM;
+  cfg.blockDim = dim3(GATHER ? G_THREADS : NUM_THREADS);
+  cfg.dynamicSmemBytes = SMEM;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -932,11 +1083,6 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   if (USES_A1) ops[n++] = &a1;
   ops[n++] = &b0;
   if (USES_B1) ops[n++] = &b1;
-  StreamMemory memory(ctx);
-  bool copied = false;
-  cudaError_t e = make_readable(ctx, memory, E, ops, n, &copied);
-  if (e != cudaSuccess) return e;
-
   Args a{};
   a.M = (int)p.M, a.N = (int)p.N;
   a.nkb = (int)((p.K + T::BK - 1) / T::BK);
@@ -944,7 +1090,6 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   a.row_scale = p.row_scale, a.col_scale = p.col_scale, a.col_scale1 = p.col_scale1, a.bias = p.bias;
   a.c0 = p.c0, a.c1 = p.c1, a.c2 = p.c2;
   a.status = ctx->status_dev;
-  a.b_early = copied ? 0 : 1;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p.c0) | reinterpret_cast<uintptr_t>(p.c1) |
                          reinterpret_cast<uintptr_t>(p.c2);
   const int Z = KIND == WGRAD ? 2 : 1;
@@ -953,6 +1098,27 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
     a.tiles_n = (int)((p.N + cols - 1) / cols);
     return (int64_t)a.tiles_m * a.tiles_n * Z;
   };
+  if constexpr (!T::B_MN) {
+    bool readable = true;
+    for (int i = 0; i < n; i++) readable = readable && ops[i]->pitch % 16 == 0 && aligned16(ops[i]->base);
+    if (!readable && gather_wanted(p.M) && p.K * E < INT32_MAX - 1024) {
+      const int64_t tiles = tiles_of(BM, T::TWO ? 64 : 128);
+      if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+      a.a_rows = (int)std::min<int64_t>(BM, (p.M + 7) / 8 * 8);
+      a.vec = p.N % 4 == 0 && bits % (4 * sizeof(O)) == 0;
+      a.a = static_cast<const uint8_t*>(p.a0);
+      a.b = static_cast<const uint8_t*>(p.b0), a.b1 = static_cast<const uint8_t*>(p.b1);
+      a.row_bytes = (int)(p.K * E);
+      CUtensorMap none[4] = {};
+      return launch_split<KIND, O, ACT, true>(ctx, none, a, tiles, after_own_kernel);
+    }
+  }
+  StreamMemory memory(ctx);
+  bool copied = false;
+  cudaError_t e = make_readable(ctx, memory, E, ops, n, &copied);
+  if (e != cudaSuccess) return e;
+
+  a.b_early = copied ? 0 : 1;
   int64_t tiles = tiles_of(2 * BM, T::TWO ? 128 : 256);
   if (tiles > INT32_MAX) return cudaErrorInvalidValue;
   if (pair_wanted(p.M, tiles)) {
@@ -982,7 +1148,7 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   if (!map_of(&maps[2], b0, E, b_rows)) return cudaErrorUnknown;
   maps[3] = maps[2];
   if (USES_B1 && !map_of(&maps[3], b1, E, b_rows)) return cudaErrorUnknown;
-  return launch_split<KIND, O, ACT>(ctx, maps, a, tiles, after_own_kernel || copied);
+  return launch_split<KIND, O, ACT, false>(ctx, maps, a, tiles, after_own_kernel || copied);
 }
 
 }  // namespace
