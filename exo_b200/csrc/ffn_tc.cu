@@ -7,7 +7,8 @@
 //
 // pair_kernel: 256 x 256 tiles on CTA pairs (cta_group::2), persistent, for problems with enough of them.  The pair's
 // B tile is half in each CTA's shared memory: for the gated kinds the even CTA loads 128 rows of the gate's weight and
-// the odd one the same 128 rows of the up projection's, and every accumulator row holds both.
+// the odd one the same 128 rows of the up projection's, and every accumulator row holds both.  Where there are few tiles
+// and a long reduction, the pairs of a cluster split it as the split kernel's CTAs do.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -48,7 +49,7 @@ struct Args {
   int tiles_m, tiles_n;
   int a_rows;            // rows of A's box (fewer than 128 when M is)
   int vec;               // outputs take vector stores
-  int b_early;           // B and the scales of its columns are not written by the kernel before this one
+  int b_early;           // the kernel before this one may still run, and writes neither B nor the scales of its columns
   const float *row_scale, *col_scale, *col_scale1, *bias;
   void *c0, *c1, *c2;
   DeviceStatus* status;
@@ -128,14 +129,18 @@ __device__ __forceinline__ void finish4(const Args& p, const Columns<KIND>& k, i
 }
 
 // ------------------------------------------------------------------ split kernel
-constexpr int S_STAGES = 3;                        // two CTAs share an SM: 2 x 3 x 32 KiB
-constexpr int S_STAGE_BYTES = 2 * A_TILE_BYTES;    // 128 rows of A, 128 of B
-constexpr int S_SMEM = S_STAGES * S_STAGE_BYTES + 1024 + 128;
+// A stage is 128 rows of B and as many of A as there are (in eights); the ring is as deep as its share of the SM takes:
+// all of it where the grid leaves an SM to each CTA, half of it otherwise.  The loads in flight are what counts: a
+// CTA alone on its SM with three stages of 32 KiB took 0.47 us a k-block, waiting for L2, 0.43 with six.
+constexpr int S_MAX_STAGES = 12;
+constexpr int S_CTRL = 1024 + 256;                 // alignment, barriers
+constexpr int S_SMEM_ALONE = 232448, S_SMEM_SHARED = 233472 / 2 - 1024;
 constexpr int S_PITCH = 132;                       // words between rows of the accumulator in shared memory: 128-bit
                                                    // accesses of neighbouring rows fall on different banks
-static_assert(BM * S_PITCH * 4 <= S_STAGES * S_STAGE_BYTES, "the accumulator takes the ring's place");
+// the accumulator takes the ring's place
+static_assert(BM * S_PITCH * 4 <= (S_SMEM_SHARED - S_CTRL) / (2 * A_TILE_BYTES) * (2 * A_TILE_BYTES), "");
 constexpr uint32_t S_TMEM_COLS = 128;
-constexpr int MAX_SPLIT = 8;
+constexpr int MAX_SPLIT = 4;
 
 __device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
   uint4 v;
@@ -149,12 +154,13 @@ template <bool I8>
 __device__ __forceinline__ uint32_t plus(uint32_t a, uint32_t b) {
   return I8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 }
-// Sum over the cluster's CTAs of the four accumulator words at `offset`, always in the order of the ranks.
-template <bool I8, int S>
-__device__ __forceinline__ void cluster_sum(uint32_t base, uint32_t offset, uint32_t (&x)[4]) {
+// Sum over S CTAs of the cluster, of ranks first, first + RANKS, ..., of the four accumulator words at `offset`; always
+// in the order of the ranks.
+template <bool I8, int S, int RANKS>
+__device__ __forceinline__ void cluster_sum(uint32_t base, uint32_t offset, int first, uint32_t (&x)[4]) {
   uint4 v[S];
 #pragma unroll
-  for (int s = 0; s < S; s++) v[s] = ld_cluster_v4(mapa(base, s) + offset);
+  for (int s = 0; s < S; s++) v[s] = ld_cluster_v4(mapa(base, (uint32_t)(first + s * RANKS)) + offset);
   x[0] = v[0].x, x[1] = v[0].y, x[2] = v[0].z, x[3] = v[0].w;
 #pragma unroll
   for (int s = 1; s < S; s++) {
@@ -165,33 +171,36 @@ __device__ __forceinline__ void cluster_sum(uint32_t base, uint32_t offset, uint
   }
 }
 
-// Rows rank, rank + S, ... of the tile: sums over the cluster, epilogue, stores.  A thread keeps its four columns and
-// goes down the rows, several at a time so that their shared-memory round trips overlap.
-template <int KIND, class O, int ACT, int THREADS, int S>
-__device__ __forceinline__ void split_epilogue(const Args& p, uint32_t base, int rank, int z, int m0, int n0) {
+// Rows split, split + S, ... of a CTA's 128 (from m0): sums over the cluster, epilogue, stores.  The accumulators lie in
+// shared memory, COLS columns in rows of PITCH words.  A thread keeps its four columns and goes down the rows, several
+// at a time so that their round trips overlap.
+template <int KIND, class O, int ACT, int THREADS, int S, int COLS, int PITCH, int RANKS>
+__device__ __forceinline__ void cluster_epilogue(const Args& p, uint32_t base, int split, int first_rank, int z, int m0,
+                                                 int n0) {
   using T = Traits<KIND>;
-  constexpr int GROUPS = T::TWO ? 16 : 32;        // groups of four output columns
-  constexpr int STEP = THREADS / GROUPS;          // rows that the CTA covers at a time
+  constexpr int GROUPS = (T::TWO ? COLS / 2 : COLS) / 4;  // groups of four output columns
+  constexpr int STEP = THREADS / GROUPS;                  // rows that the CTA covers at a time
   constexpr int BATCH = S > 2 ? 2 : 4;
+  static_assert(THREADS % GROUPS == 0, "a thread keeps its columns");
   const Columns<KIND> cols(p, n0 + (int)threadIdx.x % GROUPS * 4);
   if (cols.left <= 0) return;
-  const int rows = (min(BM, p.M - m0) - rank + S - 1) / S;
+  const int rows = (min(BM, p.M - m0) - split + S - 1) / S;
   const uint32_t c = (uint32_t)threadIdx.x % GROUPS * 16u;
   for (int first = threadIdx.x / GROUPS; first < rows; first += STEP * BATCH) {
     uint32_t x[BATCH][4], y[BATCH][4] = {};
     float rs[BATCH] = {};
 #pragma unroll
     for (int b = 0; b < BATCH; b++) {
-      const int r = rank + min(first + b * STEP, rows - 1) * S;
+      const int r = split + min(first + b * STEP, rows - 1) * S;
       if constexpr (T::I8) rs[b] = p.row_scale[m0 + r];
-      const uint32_t at = (uint32_t)(r * S_PITCH) * 4u + c;
-      cluster_sum<T::I8, S>(base, at, x[b]);
-      if constexpr (T::TWO) cluster_sum<T::I8, S>(base, at + 64 * 4, y[b]);
+      const uint32_t at = (uint32_t)(r * PITCH) * 4u + c;
+      cluster_sum<T::I8, S, RANKS>(base, at, first_rank, x[b]);
+      if constexpr (T::TWO) cluster_sum<T::I8, S, RANKS>(base, at + COLS / 2 * 4, first_rank, y[b]);
     }
 #pragma unroll
     for (int b = 0; b < BATCH; b++)
       if (first + b * STEP < rows)
-        finish4<KIND, O, ACT>(p, cols, z, m0 + rank + (first + b * STEP) * S, rs[b], x[b], y[b]);
+        finish4<KIND, O, ACT>(p, cols, z, m0 + split + (first + b * STEP) * S, rs[b], x[b], y[b]);
   }
 }
 
@@ -208,9 +217,9 @@ constexpr int G_DEPTH = 3;                      // raw k-blocks, two of them in 
 constexpr int G_A_TILE = G_MAX_M * ROW_BYTES, G_STAGE_BYTES = G_A_TILE + A_TILE_BYTES;
 constexpr int G_RAW = (G_MAX_M + BM) * G_RAW_ROW;
 constexpr int G_AREA = G_STAGES * G_STAGE_BYTES + G_DEPTH * G_RAW;
-constexpr int G_SMEM = G_AREA + 1024 + 128;
+constexpr int G_SMEM = G_AREA + S_CTRL;
 static_assert(G_AREA >= BM * S_PITCH * 4, "the accumulator takes the rings' place");
-static_assert(2 * (G_SMEM + 1024) <= 233472, "two CTAs share an SM");
+static_assert(G_SMEM <= S_SMEM_SHARED, "two CTAs share an SM");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
   const int bytes = in ? 16 : 0;  // zeros otherwise
@@ -329,7 +338,7 @@ template <int KIND, class O, int ACT, bool GATHER>
 __global__ void __launch_bounds__(GATHER ? G_THREADS : NUM_THREADS, 2)
 split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
              const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
-             const __grid_constant__ Args p, int S) {
+             const __grid_constant__ Args p, int S, int ring_stages) {
   using T = Traits<KIND>;
   constexpr int BK = T::BK;
   constexpr int CN = T::TWO ? 64 : 128;  // output columns of a tile
@@ -339,15 +348,17 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t tiles = (raw + 1023u) & ~1023u;
-  constexpr int STAGES = GATHER ? G_STAGES : S_STAGES;
-  constexpr int A_TILE = GATHER ? G_A_TILE : A_TILE_BYTES, STAGE_BYTES = A_TILE + A_TILE_BYTES;
-  const uint32_t bars = tiles + (GATHER ? G_AREA : S_STAGES * S_STAGE_BYTES);
+  const int stages = GATHER ? G_STAGES : ring_stages;
+  // The MMA reads 128 rows of A whatever there are: those behind a_rows are B's bytes, and their sums are not stored.
+  const int a_tile = GATHER ? G_A_TILE : T::A_MN ? A_TILE_BYTES : p.a_rows * ROW_BYTES;
+  const int stage_bytes = a_tile + A_TILE_BYTES;
+  const uint32_t bars = tiles + (GATHER ? G_AREA : stages * stage_bytes);
   uint8_t* ctrl = smem_raw + (bars - raw);
   auto full_bar = [&](int s) { return bars + 8u * s; };
-  auto empty_bar = [&](int s) { return bars + 8u * (S_STAGES + s); };
-  const uint32_t done_bar = bars + 8u * (2 * S_STAGES);
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl + 8 * (2 * S_STAGES + 1));
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * S_STAGES + 1) + 4);
+  auto empty_bar = [&](int s) { return bars + 8u * (S_MAX_STAGES + s); };
+  const uint32_t done_bar = bars + 8u * (2 * S_MAX_STAGES);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl + 8 * (2 * S_MAX_STAGES + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * S_MAX_STAGES + 1) + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)blockIdx.x % S;  // the cluster is S consecutive CTAs
@@ -360,7 +371,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
   const int kb0 = (int)((int64_t)total * rank / S), n_kb = (int)((int64_t)total * (rank + 1) / S) - kb0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S_STAGES; s++) {
+    for (int s = 0; s < stages; s++) {
       mbar_init(full_bar(s), GATHER ? G_WARPS : 1);
       mbar_init(empty_bar(s), 1);
     }
@@ -386,12 +397,12 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
 
   if (warp == 0) {
     if (!GATHER && lane == 0) {
-      const uint32_t a_bytes = T::A_MN ? (uint32_t)A_TILE_BYTES : (uint32_t)p.a_rows * ROW_BYTES;
+      const uint32_t a_bytes = (uint32_t)a_tile;
       auto load_a = [&](int s, int kb) {
         const bool second = kb >= p.nkb;
         const int k0 = (second ? kb - p.nkb : kb) * BK;
         const CUtensorMap* m = second || (KIND == WGRAD && z) ? &tmA1 : &tmA0;
-        const uint32_t dst = tiles + s * S_STAGE_BYTES;
+        const uint32_t dst = tiles + s * stage_bytes;
         if (T::A_MN) {
           for (int c = 0; c < 2; c++) tma_load_2d(dst + c * (A_TILE_BYTES / 2), m, full_bar(s), m0 + 64 * c, k0);
         } else {
@@ -401,7 +412,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
       auto load_b = [&](int s, int kb) {
         const bool second = kb >= p.nkb;
         const int k0 = (second ? kb - p.nkb : kb) * BK;
-        const uint32_t dst = tiles + s * S_STAGE_BYTES + A_TILE_BYTES;
+        const uint32_t dst = tiles + s * stage_bytes + a_tile;
         if (T::TWO) {
           tma_load_2d(dst, &tmB0, full_bar(s), k0, n0);
           tma_load_2d(dst + A_TILE_BYTES / 2, &tmB1, full_bar(s), k0, n0);
@@ -412,13 +423,24 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
           tma_load_2d(dst, &tmB0, full_bar(s), k0, n0);
         }
       };
-      // The ring's first fill: what the kernel before this one does not write comes before waiting for that kernel.
-      const int first = min(n_kb, S_STAGES);
-      for (int i = 0; i < first; i++) mbar_arrive_expect_tx(full_bar(i), a_bytes + A_TILE_BYTES);
-      if (!p.b_early) grid_dep_wait();
-      for (int i = 0; i < first; i++) load_b(i, kb0 + i);
-      if (p.b_early) grid_dep_wait();
-      for (int i = 0; i < first; i++) load_a(i, kb0 + i);
+      // The ring's first fill.  Beside a kernel of this call, what that kernel does not write comes before waiting for
+      // it; otherwise stage by stage, as the MMAs want it.
+      const int first = min(n_kb, stages);
+      if (p.b_early) {
+        for (int i = 0; i < first; i++) {
+          mbar_arrive_expect_tx(full_bar(i), a_bytes + A_TILE_BYTES);
+          load_b(i, kb0 + i);
+        }
+        grid_dep_wait();
+        for (int i = 0; i < first; i++) load_a(i, kb0 + i);
+      } else {
+        grid_dep_wait();
+        for (int i = 0; i < first; i++) {
+          mbar_arrive_expect_tx(full_bar(i), a_bytes + A_TILE_BYTES);
+          load_b(i, kb0 + i);
+          load_a(i, kb0 + i);
+        }
+      }
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -431,7 +453,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
         mbar_arrive_expect_tx(full_bar(stage), a_bytes + A_TILE_BYTES);
         load_b(stage, kb0 + i);
         load_a(stage, kb0 + i);
-        if (++stage == S_STAGES) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
@@ -455,14 +477,14 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
           break;
         }
         tc_fence_after();
-        const uint32_t a0 = tiles + stage * STAGE_BYTES, b0 = a0 + A_TILE;
+        const uint32_t a0 = tiles + stage * stage_bytes, b0 = a0 + a_tile;
         const uint64_t da = T::A_MN ? smem_desc_mn_sw128(a0, BK) : smem_desc_k_sw128(a0);
         const uint64_t db = T::B_MN ? smem_desc_mn_sw128(b0, BK) : smem_desc_k_sw128(b0);
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ks++)
           tc_mma<T::MMA>(tmem, da + ks * T::step(T::A_MN), db + ks * T::step(T::B_MN), IDESC, (i | ks) != 0);
         tc_commit(empty_bar(stage));
-        if (++stage == STAGES) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
@@ -505,13 +527,11 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
   else
     __syncthreads();
   if (S == 1)
-    split_epilogue<KIND, O, ACT, THREADS, 1>(p, tiles, rank, z, m0, n0);
+    cluster_epilogue<KIND, O, ACT, THREADS, 1, 128, S_PITCH, 1>(p, tiles, rank, 0, z, m0, n0);
   else if (S == 2)
-    split_epilogue<KIND, O, ACT, THREADS, 2>(p, tiles, rank, z, m0, n0);
-  else if (S == 4)
-    split_epilogue<KIND, O, ACT, THREADS, 4>(p, tiles, rank, z, m0, n0);
+    cluster_epilogue<KIND, O, ACT, THREADS, 2, 128, S_PITCH, 1>(p, tiles, rank, 0, z, m0, n0);
   else
-    split_epilogue<KIND, O, ACT, THREADS, 8>(p, tiles, rank, z, m0, n0);
+    cluster_epilogue<KIND, O, ACT, THREADS, 4, 128, S_PITCH, 1>(p, tiles, rank, 0, z, m0, n0);
   if (S > 1) cluster_sync_all();  // shared memory stays until every CTA of the cluster has read it
   if (warp == 1) {
     tc_fence_after();
@@ -530,6 +550,8 @@ constexpr int P_SMEM = P_CTRL + 1024 + 256;
 static_assert(P_SMEM <= 232448, "exceeds the shared memory a CTA can opt in to");
 constexpr int PN = 256;                           // accumulator columns of a tile
 constexpr uint32_t P_TMEM_COLS = 512;             // two accumulators
+constexpr int P_PITCH = PN + 4;                   // words between accumulator rows in shared memory, as S_PITCH
+static_assert(BM * P_PITCH * 4 <= P_STAGES * P_STAGE_BYTES, "the accumulator takes the ring's place");
 
 struct PairMaps {
   CUtensorMap a0, a1, b0, b1, c0, c1, c2;
@@ -607,7 +629,8 @@ __device__ __forceinline__ void pack(const float (&v)[32], uint32_t (&w)[W]) {
   }
 }
 
-template <int KIND, class O, int ACT>
+// SPLIT: one tile for each cluster of two pairs; otherwise persistent over the tiles, in groups of group_rows.
+template <int KIND, class O, int ACT, bool SPLIT>
 __global__ void __launch_bounds__(P_THREADS, 1)
 pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args p, int group_rows) {
   using T = Traits<KIND>;
@@ -629,8 +652,11 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
   volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * P_STAGES + 4) + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();  // 0: owns full[] and tempty[], issues the MMAs
-  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const uint32_t cluster_rank = cluster_ctarank(), rank = cluster_rank & 1u;  // even: owns full[] and tempty[], issues
+  const uint32_t even = cluster_rank & ~1u;
+  const int split = SPLIT ? (int)(cluster_rank >> 1) : 0;
+  constexpr int splits = SPLIT ? 2 : 1;
+  const int pair = (int)blockIdx.x / (2 * splits);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < P_STAGES; s++) {
@@ -662,7 +688,9 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
 
   const int per_z = p.tiles_m * p.tiles_n;
   const int num_tiles = per_z * (KIND == WGRAD ? 2 : 1);
+  const int num_pairs = SPLIT ? num_tiles : (int)gridDim.x >> 1;  // (SPLIT: one tile for each)
   const int total = p.nkb * p.segments;
+  const int kb0 = SPLIT && split ? total / 2 : 0, kb1 = SPLIT && split == 0 ? total / 2 : total;
   auto tile_coord = [&](int t, int& z, int& tm, int& tn) {
     z = t / per_z;
     t -= z * per_z;
@@ -673,7 +701,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
   };
   auto give_up = [&](int where) {
     report_timeout(p.status, abort_flag, where);
-    st_cluster_u32(mapa(slot_addr + 4, rank ^ 1u), 1u);  // take the partner down too
+    st_cluster_u32(mapa(slot_addr + 4, cluster_rank ^ 1u), 1u);  // take the partner down too
   };
 
   if (warp == 0) {
@@ -686,13 +714,13 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
         tile_coord(t, z, tm, tn);
         const int m0 = tm * 2 * BM + (int)rank * BM;
         const int n0 = tn * CN + (T::TWO ? 0 : (int)rank * 128);
-        for (int kb = 0; kb < total; kb++) {
+        for (int kb = kb0; kb < kb1; kb++) {
           if (!mbar_wait_relaxed(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS, 50)) {
             give_up(71);
             ok = false;
             break;
           }
-          const uint32_t bar0 = mapa(full_bar(stage), 0);
+          const uint32_t bar0 = mapa(full_bar(stage), even);
           const uint32_t a_dst = tiles + stage * P_STAGE_BYTES, b_dst = a_dst + A_TILE_BYTES;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * P_STAGE_BYTES);
           const bool second = kb >= p.nkb;
@@ -736,7 +764,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
         }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * PN);
-        for (int kb = 0; kb < total; kb++) {
+        for (int kb = kb0; kb < kb1; kb++) {
           if (!mbar_wait(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
             give_up(73);
             ok = false;
@@ -748,20 +776,42 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
           const uint64_t db = T::B_MN ? smem_desc_mn_sw128(b0, BK) : smem_desc_k_sw128(b0);
 #pragma unroll
           for (int ks = 0; ks < KSTEPS; ks++)
-            tc_mma_pair<T::MMA>(d, da + ks * T::step(T::A_MN), db + ks * T::step(T::B_MN), IDESC, (kb | ks) != 0);
-          tc_commit_pair(empty_bar(stage));
+            tc_mma_pair<T::MMA>(d, da + ks * T::step(T::A_MN), db + ks * T::step(T::B_MN), IDESC, kb != kb0 || ks != 0);
+          tc_commit_pair_at(empty_bar(stage), even);
           if (++stage == P_STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        tc_commit_pair(tfull_bar(acc));
+        tc_commit_pair_at(tfull_bar(acc), even);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
       }
     }
     __syncwarp();
+  } else if (SPLIT) {
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    const int row = q * 32 + lane;
+    if (mbar_wait_warp(tfull_bar(0), 0, abort_flag, WAIT_LIMIT_NS)) {
+      tc_fence_after();
+      // every MMA of this pair has read its operands: the ring takes the accumulator, for the other pairs to read
+#pragma unroll 1
+      for (int ch = 0; ch < 4; ch++) {
+        uint32_t r[32];
+        const int c = part * 128 + ch * 32;
+        tmem_ld_32x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
+        tmem_ld_wait();
+        const uint32_t dst = tiles + (uint32_t)(row * P_PITCH + c) * 4u;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * 16), "r"(r[4 * j]), "r"(r[4 * j + 1]),
+                       "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
+                       : "memory");
+      }
+    } else if (lane == 0) {
+      give_up(75);
+    }
   } else {
     const int q = warp & 3, part = (warp - 2) >> 2;
     BlockStore<O> store{tiles + P_STAGES * P_STAGE_BYTES + (uint32_t)(warp - 2) * P_STAGING, lane};
@@ -837,7 +887,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa(tempty_bar(acc), 0));
+      if (lane == 0) mbar_arrive_cluster(mapa(tempty_bar(acc), even));
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }
@@ -847,6 +897,13 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
 
   tc_fence_before();
   cluster_sync_all();
+  if constexpr (SPLIT) {
+    int z, tm, tn;
+    tile_coord(pair, z, tm, tn);
+    const int m0 = tm * 2 * BM + (int)rank * BM;
+    cluster_epilogue<KIND, O, ACT, P_THREADS, 2, PN, P_PITCH, 2>(p, tiles, split, (int)rank, z, m0, tn * CN);
+    cluster_sync_all();  // shared memory stays until every CTA of the cluster has read it
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc2(tmem, P_TMEM_COLS);
@@ -967,15 +1024,24 @@ bool map_of(CUtensorMap* m, const Matrix& x, int elem, int box_rows) {
                           dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Which kernel: EXOB200_FFN_PAIR=0 / 1 forces the split / the pair kernel.  Up to 128 rows the weights' bytes are what
-// counts, and the split kernel's CTAs share them out more evenly (1 x 16384 x 4096 gated: 47 against 73 us); above,
-// a pair's 256 x 256 tiles move half the operand bytes per flop (8192^3: 345 against 526 us).
-bool pair_wanted(int64_t rows, int64_t tiles) {
+// Which kernel: 0 the split kernel, 1 the persistent pair kernel, 2 the pair kernel with its reduction split over two
+// pairs.  EXOB200_FFN_PAIR=0 / 1 / 2 forces it.
+// Up to 128 rows the weights' bytes are what counts, and the split kernel's CTAs share them out more evenly
+// (1 x 16384 x 4096 gated: 47 against 73 us).  Above, a pair's 256 x 256 tile moves half the operand bytes of four
+// 128 x 128 tiles, and those come no faster than 14 TB/s out of L2 (8192^3 int8: 345 against 526 us); it wants enough
+// tiles for the pairs (int8 x 4096: 64 tiles 19.1 against 19.9 us, 32 tiles 17.0 against 15.9), or two pairs a tile and
+// a reduction long enough to share (32 tiles of 32 k-blocks: 14.0 against 15.9 us, of 8: 9.9 against 8.5; 16 tiles of
+// 32: 12.7 against 11.1).
+int pair_splits(const exo_b200_Context* ctx, int64_t rows, int64_t tiles, int k_blocks) {
   static const int mode = [] {
     const char* e = getenv("EXOB200_FFN_PAIR");
     return e ? atoi(e) : -1;
   }();
-  return mode >= 0 ? mode == 1 : rows > 128 && tiles >= 64;
+  if (mode >= 0) return std::min(std::min(mode, 2), k_blocks);
+  if (rows <= 128) return 0;
+  const int pairs = ctx->sm_count / 2;
+  if (tiles * 3 >= pairs * 2) return 1;
+  return tiles * 3 >= pairs && tiles * 2 <= pairs && k_blocks >= 24 ? 2 : 0;
 }
 
 // Operands that TMA cannot read: gathered as they are, or copied first.  Measured, gathered / copied: 16 x 16384 x 4095
@@ -994,17 +1060,21 @@ template <int KIND, class O, int ACT, bool GATHER>
 cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], const Args& a, int64_t tiles,
                          bool after_own_kernel) {
   auto* kernel = split_kernel<KIND, O, ACT, GATHER>;
-  constexpr int SMEM = GATHER ? G_SMEM : S_SMEM;
-  EXOB200_SMEM_ATTR_ONCE(kernel, SMEM, ctx->device);
+  EXOB200_SMEM_ATTR_ONCE(kernel, GATHER ? G_SMEM : S_SMEM_ALONE, ctx->device);
   const int total = a.nkb * a.segments;
-  // split the reduction while the CTAs fit the GPU at once and each keeps four k-blocks
+  // Split the reduction while every CTA has an SM to itself and two k-blocks.  (256 x 2048 x 4096 int8, 32 tiles: 14.3,
+  // 10.5, 9.5 and 14.8 us with 1, 2, 4 and 8 CTAs a tile; 512 x 2048 x 4096, 64 tiles: 14.7, 11.0, 13.0 and 26.7: past
+  // one CTA for each SM, and past four of them on one tile, adding up costs more than the shorter loops save.)
   int S = 1;
-  while (S < MAX_SPLIT && tiles * S * 2 <= 2 * ctx->sm_count && total / (2 * S) >= 4) S *= 2;
+  while (S < MAX_SPLIT && tiles * S * 2 <= ctx->sm_count && total / (2 * S) >= 2) S *= 2;
   if (tiles * S > INT32_MAX) return cudaErrorInvalidValue;
+  const int stage_bytes = (Traits<KIND>::A_MN ? A_TILE_BYTES : a.a_rows * ROW_BYTES) + A_TILE_BYTES;
+  const int room = (tiles * S <= ctx->sm_count ? S_SMEM_ALONE : S_SMEM_SHARED) - S_CTRL;
+  const int stages = std::min(S_MAX_STAGES, room / stage_bytes);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * S));
   cfg.blockDim = dim3(GATHER ? G_THREADS : NUM_THREADS);
-  cfg.dynamicSmemBytes = SMEM;
+  cfg.dynamicSmemBytes = GATHER ? G_SMEM : stages * stage_bytes + S_CTRL;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -1021,12 +1091,14 @@ cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], co
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a, S);
+  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a, S, stages);
 }
 
-template <int KIND, class O, int ACT>
-cudaError_t launch_pair(exo_b200_Context* ctx, const PairMaps& maps, const Args& a, int64_t tiles, bool after_own_kernel) {
-  auto* kernel = pair_kernel<KIND, O, ACT>;
+template <int KIND, class O, int ACT, bool SPLIT>
+cudaError_t launch_pair(exo_b200_Context* ctx, const PairMaps& maps, const Args& a, int64_t tiles,
+                        bool after_own_kernel) {
+  constexpr int splits = SPLIT ? 2 : 1;
+  auto* kernel = pair_kernel<KIND, O, ACT, SPLIT>;
   EXOB200_SMEM_ATTR_ONCE(kernel, P_SMEM, ctx->device);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(P_THREADS);
@@ -1034,20 +1106,24 @@ cudaError_t launch_pair(exo_b200_Context* ctx, const PairMaps& maps, const Args&
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = 2 * (unsigned)splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  // every instance takes a whole SM, so all of them fit as many pairs; asked once per context
-  int& max_pairs = ctx->max_ffn_pairs;
-  if (max_pairs == 0) {
-    cfg.gridDim = dim3(2 * ctx->sm_count);
-    int n = 0;
-    cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-    if (e != cudaSuccess) return e;
-    max_pairs = std::max(1, n);
+  if (SPLIT) {
+    cfg.gridDim = dim3(2 * (unsigned)(tiles * splits));
+  } else {
+    // every instance takes a whole SM, so all of them fit as many pairs; asked once per context
+    int& max_pairs = ctx->max_ffn_pairs;
+    if (max_pairs == 0) {
+      cfg.gridDim = dim3(2 * ctx->sm_count);
+      int n = 0;
+      cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+      if (e != cudaSuccess) return e;
+      max_pairs = std::max(1, n);
+    }
+    cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, max_pairs));
   }
-  cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, max_pairs));
   if (after_own_kernel) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -1118,11 +1194,12 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   cudaError_t e = make_readable(ctx, memory, E, ops, n, &copied);
   if (e != cudaSuccess) return e;
 
-  a.b_early = copied ? 0 : 1;
+  a.b_early = after_own_kernel && !copied;
   int64_t tiles = tiles_of(2 * BM, T::TWO ? 128 : 256);
   if (tiles > INT32_MAX) return cudaErrorInvalidValue;
-  if (pair_wanted(p.M, tiles)) {
-    a.vec = p.N * (int64_t)sizeof(O) % 16 == 0 && bits % 16 == 0;
+  const int splits = pair_splits(ctx, p.M, tiles, a.nkb * a.segments);
+  if (splits) {
+    a.vec = splits > 1 ? p.N % 4 == 0 && bits % (4 * sizeof(O)) == 0 : p.N * (int64_t)sizeof(O) % 16 == 0 && bits % 16 == 0;
     PairMaps m;
     if (!map_of(&m.a0, a0, E, T::A_MN ? T::BK : BM)) return cudaErrorUnknown;
     m.a1 = m.a0;
@@ -1131,10 +1208,11 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
     m.b1 = m.b0;
     if (USES_B1 && !map_of(&m.b1, b1, E, T::B_MN ? T::BK : 128)) return cudaErrorUnknown;
     m.c0 = m.c1 = m.c2 = m.a0;
-    if (a.vec && !(output_map<O>(&m.c0, p.c0, p.M, p.N) && (!p.c1 || output_map<O>(&m.c1, p.c1, p.M, p.N)) &&
+    if (a.vec && splits == 1 && !(output_map<O>(&m.c0, p.c0, p.M, p.N) && (!p.c1 || output_map<O>(&m.c1, p.c1, p.M, p.N)) &&
                    (!p.c2 || output_map<O>(&m.c2, p.c2, p.M, p.N))))
       return cudaErrorUnknown;
-    return launch_pair<KIND, O, ACT>(ctx, m, a, tiles, after_own_kernel || copied);
+    return splits > 1 ? launch_pair<KIND, O, ACT, true>(ctx, m, a, tiles, after_own_kernel || copied)
+                      : launch_pair<KIND, O, ACT, false>(ctx, m, a, tiles, after_own_kernel || copied);
   }
   tiles = tiles_of(BM, T::TWO ? 64 : 128);
   if (tiles > INT32_MAX) return cudaErrorInvalidValue;

@@ -80,6 +80,14 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
       "h"(mask)
       : "memory");
 }
+// the same for the pair whose even CTA has this rank in a cluster of several pairs
+__device__ __forceinline__ void tc_commit_pair_at(uint32_t bar, uint32_t even_rank) {
+  const uint16_t mask = (uint16_t)(3u << even_rank);
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(mask)
+      : "memory");
+}
 template <int KIND>
 __device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
