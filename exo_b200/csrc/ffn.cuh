@@ -33,6 +33,10 @@ cudaError_t launch_quantize_rows(exo_b200_Context* ctx, int64_t M, int64_t K, co
 // after_own_kernel: the kernel before this one on the stream belongs to the same call and was launched in the ordinary
 // way (or waits for one that was), so this one may be scheduled before it ends.
 cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p, bool after_own_kernel);
+// dX = dG Wg + dU Wu [M,K] and dWg = dG^T X, dWu = dU^T X [F,K], each only where it is wanted (dWg and dWu together);
+// after launch_gate_backward on the same stream.
+cudaError_t launch_gradients(exo_b200_Context* ctx, int64_t M, int64_t F, int64_t K, const void* X, const void* Wg,
+                             const void* Wu, const void* dG, const void* dU, void* dX, void* dWg, void* dWu);
 // The products of a few rows (ffn_gemv.cu): whether they are taken for a problem, and their launch.
 constexpr int kRowTokenBytes = 96 * 1024;  // tokens that a CTA keeps in shared memory
 bool rows_wanted(Kind kind, const Problem& p);

@@ -271,20 +271,9 @@ void gated_bf16_backward_exo(void* ctxt, int_fast32_t activation, int_fast32_t M
     return;
   cudaError_t e = ffn::launch_gate_backward(o.ctx(), (int)activation, M * F, o.dev<uint16_t>(3), o.dev<uint16_t>(4),
                                             o.dev<uint16_t>(5), o.dev<uint16_t>(6), o.dev<uint16_t>(7));
-  if (e == cudaSuccess && dX) {
-    ffn::Problem p{};
-    p.M = M, p.N = K, p.K = F;
-    p.a0 = o.dev<void>(6), p.a1 = o.dev<void>(7), p.b0 = o.dev<void>(1), p.b1 = o.dev<void>(2);
-    p.c0 = o.dev<void>(8);
-    e = ffn::launch_product(o.ctx(), ffn::DGRAD, false, p, true);
-  }
-  if (e == cudaSuccess && dWg) {
-    ffn::Problem p{};
-    p.M = F, p.N = K, p.K = M;
-    p.a0 = o.dev<void>(6), p.a1 = o.dev<void>(7), p.b0 = o.dev<void>(0);
-    p.c0 = o.dev<void>(9), p.c1 = o.dev<void>(10);
-    e = ffn::launch_product(o.ctx(), ffn::WGRAD, false, p, true);
-  }
+  if (e == cudaSuccess)
+    e = ffn::launch_gradients(o.ctx(), M, F, K, o.dev<void>(0), o.dev<void>(1), o.dev<void>(2), o.dev<void>(6),
+                              o.dev<void>(7), o.dev<void>(8), o.dev<void>(9), o.dev<void>(10));
   o.done(e);
 }
 

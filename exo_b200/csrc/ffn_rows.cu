@@ -69,19 +69,22 @@ __global__ void __launch_bounds__(256) quantize_vectors_kernel(int64_t M, int K,
   }
 }
 
-// Any row length and alignment: a CTA a row, element by element, the second pass out of the caches.
-template <class E>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t K, const E* X, int8_t* Q, float* scale) {
+// Any row length and alignment: a CTA or a warp a row, element by element, the second pass out of the caches.
+template <class E, int WARPS>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t M, int64_t K, const E* X, int8_t* Q, float* scale) {
   grid_dep_launch();
-  const E* x = X + (int64_t)blockIdx.x * K;
-  int8_t* q = Q + (int64_t)blockIdx.x * K;
+  const int64_t row = (int64_t)blockIdx.x * (8 / WARPS) + (WARPS == 8 ? 0 : threadIdx.x / 32);
+  const int t = threadIdx.x % (32 * WARPS);
+  if (WARPS == 1 && row >= M) return;
+  const E* x = X + row * K;
+  int8_t* q = Q + row * K;
   unsigned top = 0;
 #pragma unroll 8
-  for (int64_t k = threadIdx.x; k < K; k += 256) top = max(top, magnitude(float(x[k])));
-  const Step s = step_of(row_top<8>(top));
-  if (threadIdx.x == 0) scale[blockIdx.x] = s.scale;
+  for (int64_t k = t; k < K; k += 32 * WARPS) top = max(top, magnitude(float(x[k])));
+  const Step s = step_of(row_top<WARPS>(top));
+  if (t == 0) scale[row] = s.scale;
 #pragma unroll 8
-  for (int64_t k = threadIdx.x; k < K; k += 256) q[k] = (int8_t)quantized(float(x[k]), s);
+  for (int64_t k = t; k < K; k += 32 * WARPS) q[k] = (int8_t)quantized(float(x[k]), s);
 }
 
 template <class E>
@@ -101,8 +104,10 @@ cudaError_t quantize(exo_b200_Context* ctx, int64_t M, int64_t K, const E* X, in
     quantize_vectors_kernel<E, 4, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
   else if (vectors && K <= 2048 * N)
     quantize_vectors_kernel<E, 8, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
+  else if (K <= 1024 && M >= 8 * ctx->sm_count)
+    quantize_rows_kernel<E, 1><<<(m + 7) / 8, 256, 0, st>>>(M, K, X, Q, scale);
   else
-    quantize_rows_kernel<E><<<m, 256, 0, st>>>(K, X, Q, scale);
+    quantize_rows_kernel<E, 8><<<m, 256, 0, st>>>(M, K, X, Q, scale);
   return cudaGetLastError();
 }
 

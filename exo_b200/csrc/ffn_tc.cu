@@ -50,12 +50,20 @@ struct Args {
   int a_rows;            // rows of A's box (fewer than 128 when M is)
   int vec;               // outputs take vector stores
   int b_early;           // the kernel before this one may still run, and writes neither B nor the scales of its columns
+  int let_beside;        // successors may start once this kernel has what it waits for
+  int wait_last;         // beside the kernel before it: waits for that one only before it ends
   const float *row_scale, *col_scale, *col_scale1, *bias;
   void *c0, *c1, *c2;
   DeviceStatus* status;
   const uint8_t *a, *b, *b1;  // operands that are gathered instead of copied by TMA; rows of row_bytes
   int row_bytes;
 };
+
+// What the kernel before this one wrote may be read from here on.
+__device__ __forceinline__ void wait_before(const Args& p) {
+  if (!p.wait_last) grid_dep_wait();
+  if (p.let_beside) grid_dep_launch();
+}
 
 // ------------------------------------------------------------------ epilogue arithmetic
 template <class O>
@@ -140,7 +148,7 @@ constexpr int S_PITCH = 132;                       // words between rows of the 
 // the accumulator takes the ring's place
 static_assert(BM * S_PITCH * 4 <= (S_SMEM_SHARED - S_CTRL) / (2 * A_TILE_BYTES) * (2 * A_TILE_BYTES), "");
 constexpr uint32_t S_TMEM_COLS = 128;
-constexpr int MAX_SPLIT = 4;
+constexpr int MAX_SPLIT = 16;  // CTAs of a cluster; above eight the size is not portable, but this GPU takes it
 
 __device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
   uint4 v;
@@ -180,7 +188,7 @@ __device__ __forceinline__ void cluster_epilogue(const Args& p, uint32_t base, i
   using T = Traits<KIND>;
   constexpr int GROUPS = (T::TWO ? COLS / 2 : COLS) / 4;  // groups of four output columns
   constexpr int STEP = THREADS / GROUPS;                  // rows that the CTA covers at a time
-  constexpr int BATCH = S > 2 ? 2 : 4;
+  constexpr int BATCH = S > 4 ? 1 : S > 2 ? 2 : 4;
   static_assert(THREADS % GROUPS == 0, "a thread keeps its columns");
   const Columns<KIND> cols(p, n0 + (int)threadIdx.x % GROUPS * 4);
   if (cols.left <= 0) return;
@@ -431,10 +439,10 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
           mbar_arrive_expect_tx(full_bar(i), a_bytes + A_TILE_BYTES);
           load_b(i, kb0 + i);
         }
-        grid_dep_wait();
+        wait_before(p);
         for (int i = 0; i < first; i++) load_a(i, kb0 + i);
       } else {
-        grid_dep_wait();
+        wait_before(p);
         for (int i = 0; i < first; i++) {
           mbar_arrive_expect_tx(full_bar(i), a_bytes + A_TILE_BYTES);
           load_b(i, kb0 + i);
@@ -495,7 +503,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
   } else {
     const int q = warp & 3;  // a warp reads the 32 tensor-memory lanes of its quarter
     const int row = q * 32 + lane;
-    grid_dep_wait();  // the row scales may be the preceding kernel's
+    wait_before(p);  // the row scales may be the preceding kernel's
     if constexpr (GATHER)
       gather<KIND>(p, tiles, full_bar(0), empty_bar(0), abort_flag, warp - 2, lane, m0, n0, kb0, n_kb);
     if (warp < 6 && mbar_wait_warp(done_bar, 0, abort_flag, WAIT_LIMIT_NS)) {
@@ -521,7 +529,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
     }
   }
   // warps 0 and 1 read what the preceding kernel wrote in the epilogue, too
-  if (warp < 2) grid_dep_wait();
+  if (warp < 2) wait_before(p);
   if (S > 1)
     cluster_sync_all();
   else
@@ -530,13 +538,18 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
     cluster_epilogue<KIND, O, ACT, THREADS, 1, 128, S_PITCH, 1>(p, tiles, rank, 0, z, m0, n0);
   else if (S == 2)
     cluster_epilogue<KIND, O, ACT, THREADS, 2, 128, S_PITCH, 1>(p, tiles, rank, 0, z, m0, n0);
-  else
+  else if (S == 4)
     cluster_epilogue<KIND, O, ACT, THREADS, 4, 128, S_PITCH, 1>(p, tiles, rank, 0, z, m0, n0);
+  else if (S == 8)
+    cluster_epilogue<KIND, O, ACT, THREADS, 8, 128, S_PITCH, 1>(p, tiles, rank, 0, z, m0, n0);
+  else
+    cluster_epilogue<KIND, O, ACT, THREADS, 16, 128, S_PITCH, 1>(p, tiles, rank, 0, z, m0, n0);
   if (S > 1) cluster_sync_all();  // shared memory stays until every CTA of the cluster has read it
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, S_TMEM_COLS);
   }
+  if (p.wait_last) grid_dep_wait();
 }
 
 // ------------------------------------------------------------------ pair kernel
@@ -684,7 +697,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  grid_dep_wait();
+  wait_before(p);
 
   const int per_z = p.tiles_m * p.tiles_n;
   const int num_tiles = per_z * (KIND == WGRAD ? 2 : 1);
@@ -908,6 +921,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
     tc_fence_after();
     tmem_dealloc2(tmem, P_TMEM_COLS);
   }
+  if (p.wait_last) grid_dep_wait();
 }
 
 // ------------------------------------------------------------------ operand copies with a pitch that TMA takes
@@ -918,7 +932,7 @@ struct PadJob {
   uint8_t* dst;
   int64_t rows, src_pitch, dst_pitch;
 };
-constexpr int kMaxPads = 4;
+constexpr int kMaxPads = 5;
 struct PadJobs {
   PadJob job[kMaxPads];
 };
@@ -1024,24 +1038,41 @@ bool map_of(CUtensorMap* m, const Matrix& x, int elem, int box_rows) {
                           dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// How many CTAs of the split kernel share a tile's reduction: as long as every CTA has an SM to itself and two k-blocks.
+// (256 x 2048 x 4096 int8, 32 tiles: 14.3, 10.5, 9.5 and 14.8 us with 1, 2, 4 and 8 CTAs a tile; 512 x 2048 x 4096, 64
+// tiles: 14.7, 11.0, 13.0 and 26.7: past one CTA for each SM, and mostly past four of them on one tile, adding up costs
+// more than the shorter loops save.)  A handful of tiles with a long reduction splits further (the gradient of 3 x 177
+// inputs over 2 x 14054 units, two tiles: FILL_S4 us with four, 12.8 with sixteen).
+int split_of(const exo_b200_Context* ctx, int64_t tiles, int k_blocks) {
+  int S = 1;
+  while (S < 4 && tiles * S * 2 <= ctx->sm_count && k_blocks / (2 * S) >= 2) S *= 2;
+  while (S >= 4 && S < MAX_SPLIT && tiles * S * 4 <= ctx->sm_count && k_blocks / (2 * S) >= 8) S *= 2;
+  return S;
+}
+
 // Which kernel: 0 the split kernel, 1 the persistent pair kernel, 2 the pair kernel with its reduction split over two
 // pairs.  EXOB200_FFN_PAIR=0 / 1 / 2 forces it.
 // Up to 128 rows the weights' bytes are what counts, and the split kernel's CTAs share them out more evenly
 // (1 x 16384 x 4096 gated: 47 against 73 us).  Above, a pair's 256 x 256 tile moves half the operand bytes of four
-// 128 x 128 tiles, and those come no faster than 14 TB/s out of L2 (8192^3 int8: 345 against 526 us); it wants enough
-// tiles for the pairs (int8 x 4096: 64 tiles 19.1 against 19.9 us, 32 tiles 17.0 against 15.9), or two pairs a tile and
-// a reduction long enough to share (32 tiles of 32 k-blocks: 14.0 against 15.9 us, of 8: 9.9 against 8.5; 16 tiles of
-// 32: 12.7 against 11.1).
-int pair_splits(const exo_b200_Context* ctx, int64_t rows, int64_t tiles, int k_blocks) {
+// 128 x 128 tiles, which come no faster than 14 TB/s out of L2 (8192^3 int8: 345 against 526 us).  Below a full round
+// of tiles the time is a fixed part and so much for each k-block that one CTA goes through: fitted, in us, on products
+// and gated products of 160 to 2048 rows, 512 to 8192 columns and 2 to 64 k-blocks (split / pair / two pairs measured:
+// 1024 x 1024 x 1024 int8 7.6 / 9.5 / 9.3, 1024 x 4096 x 4096 19.9 / 19.1 / 28, 512 x 4096 x 4096 15.9 / 17.0 / 14.0).
+int pair_splits(const exo_b200_Context* ctx, int64_t rows, int64_t pair_tiles, int64_t split_tiles, int k_blocks) {
   static const int mode = [] {
     const char* e = getenv("EXOB200_FFN_PAIR");
     return e ? atoi(e) : -1;
   }();
   if (mode >= 0) return std::min(std::min(mode, 2), k_blocks);
   if (rows <= 128) return 0;
-  const int pairs = ctx->sm_count / 2;
-  if (tiles * 3 >= pairs * 2) return 1;
-  return tiles * 3 >= pairs && tiles * 2 <= pairs && k_blocks >= 24 ? 2 : 0;
+  const int S = split_of(ctx, split_tiles, k_blocks), sms = ctx->sm_count, pairs = sms / 2;
+  auto rounds = [](int64_t work, int64_t slots) { return (double)((work + slots - 1) / slots); };
+  const bool alone = split_tiles * S <= sms;
+  const double loop = rounds(k_blocks, S);
+  const double split = 5.2 + (alone ? 0.30 * loop + (S > 1 ? 0.5 : 0.0) : 0.46 * loop * rounds(split_tiles, 2 * sms));
+  const double pair = 6.0 + 0.31 * k_blocks * rounds(pair_tiles, pairs);
+  const double two = pair_tiles * 2 <= pairs && k_blocks >= 2 ? 8.0 + 0.34 * rounds(k_blocks, 2) : 1e30;
+  return split <= pair && split <= two ? 0 : pair <= two ? 1 : 2;
 }
 
 // Operands that TMA cannot read: gathered as they are, or copied first.  Measured, gathered / copied: 16 x 16384 x 4095
@@ -1062,12 +1093,17 @@ cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], co
   auto* kernel = split_kernel<KIND, O, ACT, GATHER>;
   EXOB200_SMEM_ATTR_ONCE(kernel, GATHER ? G_SMEM : S_SMEM_ALONE, ctx->device);
   const int total = a.nkb * a.segments;
-  // Split the reduction while every CTA has an SM to itself and two k-blocks.  (256 x 2048 x 4096 int8, 32 tiles: 14.3,
-  // 10.5, 9.5 and 14.8 us with 1, 2, 4 and 8 CTAs a tile; 512 x 2048 x 4096, 64 tiles: 14.7, 11.0, 13.0 and 26.7: past
-  // one CTA for each SM, and past four of them on one tile, adding up costs more than the shorter loops save.)
-  int S = 1;
-  while (S < MAX_SPLIT && tiles * S * 2 <= ctx->sm_count && total / (2 * S) >= 2) S *= 2;
+  const int S = split_of(ctx, tiles, total);
   if (tiles * S > INT32_MAX) return cudaErrorInvalidValue;
+  if (S > 8) {
+    static std::atomic<uint64_t> allowed{0};
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (!(allowed.load(std::memory_order_acquire) & bit)) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+      allowed.fetch_or(bit, std::memory_order_release);
+    }
+  }
   const int stage_bytes = (Traits<KIND>::A_MN ? A_TILE_BYTES : a.a_rows * ROW_BYTES) + A_TILE_BYTES;
   const int room = (tiles * S <= ctx->sm_count ? S_SMEM_ALONE : S_SMEM_SHARED) - S_CTRL;
   const int stages = std::min(S_MAX_STAGES, room / stage_bytes);
@@ -1143,22 +1179,21 @@ bool output_map(CUtensorMap* m, void* base, int64_t rows, int64_t cols) {
                           sizeof(O) == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// How a product stands to the kernel before it on the stream.
+enum After {
+  OTHERS,  // anything: wait for it in the ordinary way
+  OWN,     // a kernel of the same call, itself ordered after everything earlier: this one may be scheduled beside it and
+           // waits for it before reading what it writes
+  BESIDE   // a product that was launched OWN and let its successors start: this one reads nothing of it, runs beside it
+           // and only ends after it
+};
+
 template <int KIND, class O, int ACT>
-cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kernel) {
+cudaError_t run(exo_b200_Context* ctx, const Problem& p, const Matrix& a0, const Matrix& a1, const Matrix& b0,
+                const Matrix& b1, After after, bool b_copied, bool let_beside) {
   using T = Traits<KIND>;
   constexpr int E = T::ELEM;
-  auto matrix = [](const void* base, int64_t rows, int64_t width) { return Matrix{base, rows, width, width * E}; };
-  Matrix a0 = T::A_MN ? matrix(p.a0, p.K, p.M) : matrix(p.a0, p.M, p.K), a1 = a0;
-  a1.base = p.a1;
-  Matrix b0 = T::B_MN ? matrix(p.b0, p.K, p.N) : matrix(p.b0, p.N, p.K), b1 = b0;
-  b1.base = p.b1;
   constexpr bool USES_A1 = KIND == WGRAD || KIND == DGRAD, USES_B1 = T::TWO || KIND == DGRAD;
-  Matrix* ops[4];
-  int n = 0;
-  ops[n++] = &a0;
-  if (USES_A1) ops[n++] = &a1;
-  ops[n++] = &b0;
-  if (USES_B1) ops[n++] = &b1;
   Args a{};
   a.M = (int)p.M, a.N = (int)p.N;
   a.nkb = (int)((p.K + T::BK - 1) / T::BK);
@@ -1166,6 +1201,9 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   a.row_scale = p.row_scale, a.col_scale = p.col_scale, a.col_scale1 = p.col_scale1, a.bias = p.bias;
   a.c0 = p.c0, a.c1 = p.c1, a.c2 = p.c2;
   a.status = ctx->status_dev;
+  a.b_early = after == OWN && !b_copied;
+  a.wait_last = after == BESIDE;
+  a.let_beside = let_beside;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p.c0) | reinterpret_cast<uintptr_t>(p.c1) |
                          reinterpret_cast<uintptr_t>(p.c2);
   const int Z = KIND == WGRAD ? 2 : 1;
@@ -1174,59 +1212,71 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
     a.tiles_n = (int)((p.N + cols - 1) / cols);
     return (int64_t)a.tiles_m * a.tiles_n * Z;
   };
+  const bool any4 = p.N % 4 == 0 && bits % (4 * sizeof(O)) == 0;  // four columns at a time
   if constexpr (!T::B_MN) {
-    bool readable = true;
-    for (int i = 0; i < n; i++) readable = readable && ops[i]->pitch % 16 == 0 && aligned16(ops[i]->base);
-    if (!readable && gather_wanted(p.M) && p.K * E < INT32_MAX - 1024) {
+    auto readable = [](const Matrix& m) { return m.pitch % 16 == 0 && aligned16(m.base); };
+    if (!(readable(a0) && readable(b0) && (!USES_B1 || readable(b1)))) {  // only left as they are to be gathered
       const int64_t tiles = tiles_of(BM, T::TWO ? 64 : 128);
       if (tiles > INT32_MAX) return cudaErrorInvalidValue;
       a.a_rows = (int)std::min<int64_t>(BM, (p.M + 7) / 8 * 8);
-      a.vec = p.N % 4 == 0 && bits % (4 * sizeof(O)) == 0;
-      a.a = static_cast<const uint8_t*>(p.a0);
-      a.b = static_cast<const uint8_t*>(p.b0), a.b1 = static_cast<const uint8_t*>(p.b1);
+      a.vec = any4;
+      a.a = static_cast<const uint8_t*>(a0.base);
+      a.b = static_cast<const uint8_t*>(b0.base), a.b1 = static_cast<const uint8_t*>(b1.base);
       a.row_bytes = (int)(p.K * E);
       CUtensorMap none[4] = {};
-      return launch_split<KIND, O, ACT, true>(ctx, none, a, tiles, after_own_kernel);
+      return launch_split<KIND, O, ACT, true>(ctx, none, a, tiles, after != OTHERS);
     }
   }
-  StreamMemory memory(ctx);
-  bool copied = false;
-  cudaError_t e = make_readable(ctx, memory, E, ops, n, &copied);
-  if (e != cudaSuccess) return e;
-
-  a.b_early = after_own_kernel && !copied;
-  int64_t tiles = tiles_of(2 * BM, T::TWO ? 128 : 256);
-  if (tiles > INT32_MAX) return cudaErrorInvalidValue;
-  const int splits = pair_splits(ctx, p.M, tiles, a.nkb * a.segments);
+  const int64_t split_tiles = tiles_of(BM, T::TWO ? 64 : 128);
+  const int64_t pair_tiles = tiles_of(2 * BM, T::TWO ? 128 : 256);
+  if (split_tiles > INT32_MAX) return cudaErrorInvalidValue;
+  const int splits = pair_splits(ctx, p.M, pair_tiles, split_tiles, a.nkb * a.segments);
+  const int b_box = T::B_MN ? T::BK : T::TWO && !splits ? 64 : 128;
   if (splits) {
-    a.vec = splits > 1 ? p.N % 4 == 0 && bits % (4 * sizeof(O)) == 0 : p.N * (int64_t)sizeof(O) % 16 == 0 && bits % 16 == 0;
+    a.vec = splits > 1 ? any4 : p.N * (int64_t)sizeof(O) % 16 == 0 && bits % 16 == 0;
     PairMaps m;
     if (!map_of(&m.a0, a0, E, T::A_MN ? T::BK : BM)) return cudaErrorUnknown;
     m.a1 = m.a0;
     if (USES_A1 && !map_of(&m.a1, a1, E, T::A_MN ? T::BK : BM)) return cudaErrorUnknown;
-    if (!map_of(&m.b0, b0, E, T::B_MN ? T::BK : 128)) return cudaErrorUnknown;
+    if (!map_of(&m.b0, b0, E, b_box)) return cudaErrorUnknown;
     m.b1 = m.b0;
-    if (USES_B1 && !map_of(&m.b1, b1, E, T::B_MN ? T::BK : 128)) return cudaErrorUnknown;
+    if (USES_B1 && !map_of(&m.b1, b1, E, b_box)) return cudaErrorUnknown;
     m.c0 = m.c1 = m.c2 = m.a0;
-    if (a.vec && splits == 1 && !(output_map<O>(&m.c0, p.c0, p.M, p.N) && (!p.c1 || output_map<O>(&m.c1, p.c1, p.M, p.N)) &&
-                   (!p.c2 || output_map<O>(&m.c2, p.c2, p.M, p.N))))
+    if (a.vec && splits == 1 &&
+        !(output_map<O>(&m.c0, p.c0, p.M, p.N) && (!p.c1 || output_map<O>(&m.c1, p.c1, p.M, p.N)) &&
+          (!p.c2 || output_map<O>(&m.c2, p.c2, p.M, p.N))))
       return cudaErrorUnknown;
-    return splits > 1 ? launch_pair<KIND, O, ACT, true>(ctx, m, a, tiles, after_own_kernel || copied)
-                      : launch_pair<KIND, O, ACT, false>(ctx, m, a, tiles, after_own_kernel || copied);
+    return splits > 1 ? launch_pair<KIND, O, ACT, true>(ctx, m, a, pair_tiles, after != OTHERS)
+                      : launch_pair<KIND, O, ACT, false>(ctx, m, a, pair_tiles, after != OTHERS);
   }
-  tiles = tiles_of(BM, T::TWO ? 64 : 128);
-  if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+  tiles_of(BM, T::TWO ? 64 : 128);
   a.a_rows = (int)std::min<int64_t>(BM, (p.M + 7) / 8 * 8);
-  a.vec = p.N % 4 == 0 && bits % (4 * sizeof(O)) == 0;
+  a.vec = any4;
   CUtensorMap maps[4];
   if (!map_of(&maps[0], a0, E, T::A_MN ? T::BK : a.a_rows)) return cudaErrorUnknown;
   maps[1] = maps[0];
   if (USES_A1 && !map_of(&maps[1], a1, E, T::A_MN ? T::BK : a.a_rows)) return cudaErrorUnknown;
-  const int b_rows = T::B_MN ? T::BK : T::TWO ? 64 : 128;
-  if (!map_of(&maps[2], b0, E, b_rows)) return cudaErrorUnknown;
+  if (!map_of(&maps[2], b0, E, b_box)) return cudaErrorUnknown;
   maps[3] = maps[2];
-  if (USES_B1 && !map_of(&maps[3], b1, E, b_rows)) return cudaErrorUnknown;
-  return launch_split<KIND, O, ACT, false>(ctx, maps, a, tiles, after_own_kernel || copied);
+  if (USES_B1 && !map_of(&maps[3], b1, E, b_box)) return cudaErrorUnknown;
+  return launch_split<KIND, O, ACT, false>(ctx, maps, a, split_tiles, after != OTHERS);
+}
+
+// The forward kinds: A [M,K], B [N,K].
+template <int KIND, class O, int ACT>
+cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kernel) {
+  using T = Traits<KIND>;
+  constexpr int E = T::ELEM;
+  Matrix a0{p.a0, p.M, p.K, p.K * E}, b0{p.b0, p.N, p.K, p.K * E}, b1 = b0;
+  b1.base = p.b1;
+  StreamMemory memory(ctx);
+  bool copied = false;
+  if (!(gather_wanted(p.M) && p.K * E < INT32_MAX - 1024)) {
+    Matrix* ops[3] = {&a0, &b0, &b1};
+    const cudaError_t e = make_readable(ctx, memory, E, ops, T::TWO ? 3 : 2, &copied);
+    if (e != cudaSuccess) return e;
+  }
+  return run<KIND, O, ACT>(ctx, p, a0, a0, b0, b1, after_own_kernel || copied ? OWN : OTHERS, copied, false);
 }
 
 }  // namespace
@@ -1246,11 +1296,37 @@ cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const
       return p.act == 0   ? launch<GATED_I8, bf16, 0>(ctx, p, own)
              : p.act == 1 ? launch<GATED_I8, bf16, 1>(ctx, p, own)
                           : launch<GATED_I8, bf16, 2>(ctx, p, own);
-    case DGRAD:
-      return launch<DGRAD, bf16, 0>(ctx, p, own);
     default:
-      return launch<WGRAD, bf16, 0>(ctx, p, own);
+      return cudaErrorInvalidValue;  // the backward kinds go through launch_gradients
   }
+}
+
+cudaError_t launch_gradients(exo_b200_Context* ctx, int64_t M, int64_t F, int64_t K, const void* X, const void* Wg,
+                             const void* Wu, const void* dG, const void* dU, void* dX, void* dWg, void* dWu) {
+  using bf16 = __nv_bfloat16;
+  Matrix dg{dG, M, F, F * 2}, du{dU, M, F, F * 2}, x{X, M, K, K * 2}, wg{Wg, F, K, K * 2}, wu{Wu, F, K, K * 2};
+  // one pass of copies serves both products
+  Matrix* ops[5];
+  int n = 0;
+  if (dX || dWg) ops[n++] = &dg, ops[n++] = &du;
+  if (dX) ops[n++] = &wg, ops[n++] = &wu;
+  if (dWg) ops[n++] = &x;
+  StreamMemory memory(ctx);
+  bool copied = false;
+  cudaError_t e = make_readable(ctx, memory, 2, ops, n, &copied);
+  if (e == cudaSuccess && dX) {
+    Problem p{};
+    p.M = M, p.N = K, p.K = F;
+    p.c0 = dX;
+    e = run<DGRAD, bf16, 0>(ctx, p, dg, du, wg, wu, OWN, copied, dWg != nullptr);
+  }
+  if (e == cudaSuccess && dWg) {
+    Problem p{};
+    p.M = F, p.N = K, p.K = M;
+    p.c0 = dWg, p.c1 = dWu;
+    e = run<WGRAD, bf16, 0>(ctx, p, dg, du, x, x, dX ? BESIDE : OWN, copied, false);
+  }
+  return e;
 }
 
 }  // namespace ffn
