@@ -9,6 +9,8 @@
 // B tile is half in each CTA's shared memory: for the gated kinds the even CTA loads 128 rows of the gate's weight and
 // the odd one the same 128 rows of the up projection's, and every accumulator row holds both.  Where there are few tiles
 // and a long reduction, the pairs of a cluster split it as the split kernel's CTAs do.
+//
+// tall_kernel: 512 x 256 tiles on CTA pairs for the largest problems with one weight.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -574,10 +576,10 @@ struct PairMaps {
 // With a map for C: whole rows go out through the copy engine, which clips at C's edges; shared memory is
 // swizzled so that the 128-bit writes meet no bank twice.  Without (a pitch or base that TMA cannot take): rows leave
 // one by one, lane = column.
-template <class O>
+template <class O, int BUFFER>
 struct BlockStore {
   static constexpr int WORDS = sizeof(O) == 2 ? 16 : 32;
-  uint32_t area;  // this warp's staging
+  uint32_t area;  // this warp's staging: two buffers
   int lane, buf = 0;
 
   __device__ __forceinline__ void put(const uint32_t (&w)[WORDS], const CUtensorMap* m, O* C, const Args& p, int row0,
@@ -586,7 +588,7 @@ struct BlockStore {
     if (p.vec) {
       if (lane == 0) bulk_wait_read_1();  // the store that last used this buffer has read it
       __syncwarp();
-      const uint32_t at = area + (uint32_t)buf * 4096u;
+      const uint32_t at = area + (uint32_t)(buf * BUFFER);
 #pragma unroll
       for (int j = 0; j < WORDS / 4; j++) {
         const int swizzled = sizeof(O) == 2 ? j ^ ((lane >> 1) & 3) : j ^ (lane & 7);
@@ -639,6 +641,43 @@ __device__ __forceinline__ void pack(const float (&v)[32], uint32_t (&w)[W]) {
   } else {
 #pragma unroll
     for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
+  }
+}
+
+// 32 columns (from col) of one accumulator row: sums x, of the up projection y, to output values v; gated products leave
+// their pre-activations in g and u.
+template <int KIND, int ACT>
+__device__ __forceinline__ void finish32(const Args& p, const uint32_t (&x)[32], const uint32_t (&y)[32], float rs, int col,
+                                         int lane, float (&v)[32], float (&g)[32], float (&u)[32]) {
+  using T = Traits<KIND>;
+  if constexpr (T::TWO) {
+    if constexpr (T::I8) {
+      // a lane holds the scales of one column; each column's reach every row of the block by a shuffle
+      const float cg = col + lane < p.N ? __ldg(p.col_scale + col + lane) : 0.f;
+      const float cu = col + lane < p.N ? __ldg(p.col_scale1 + col + lane) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; j++) {
+        g[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, cg, j));
+        u[j] = scaled((int32_t)y[j], rs, __shfl_sync(0xffffffffu, cu, j));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j++) {
+        g[j] = __uint_as_float(x[j]);
+        u[j] = __uint_as_float(y[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = gate<ACT>(g[j]) * u[j];
+  } else if constexpr (T::I8) {
+    const float cs = col + lane < p.N ? __ldg(p.col_scale + col + lane) : 0.f;
+    const float add = p.bias && col + lane < p.N ? __ldg(p.bias + col + lane) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; j++)
+      v[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, cs, j)) + __shfl_sync(0xffffffffu, add, j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = __uint_as_float(x[j]);
   }
 }
 
@@ -827,7 +866,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
     }
   } else {
     const int q = warp & 3, part = (warp - 2) >> 2;
-    BlockStore<O> store{tiles + P_STAGES * P_STAGE_BYTES + (uint32_t)(warp - 2) * P_STAGING, lane};
+    BlockStore<O, P_STAGING / 2> store{tiles + P_STAGES * P_STAGE_BYTES + (uint32_t)(warp - 2) * P_STAGING, lane};
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = pair; t < num_tiles; t += num_pairs) {
@@ -847,50 +886,17 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
 #pragma unroll 1
       for (int ch = 0; ch < CN / 64; ch++) {
         const int col = c0 + ch * 32;
-        uint32_t x[32], w[BlockStore<O>::WORDS];
-        float v[32];
+        uint32_t x[32], y[32], w[BlockStore<O, P_STAGING / 2>::WORDS];
+        float v[32], g[32], u[32];
         tmem_ld_32x32(from + (uint32_t)(ch * 32), x);
-        if constexpr (T::TWO) {
-          uint32_t y[32];
-          float u[32];
-          tmem_ld_32x32(from + (uint32_t)(128 + ch * 32), y);
-          tmem_ld_wait();
-          if constexpr (T::I8) {
-            // a lane holds the scales of one column; each column's reach every row of the block by a shuffle
-            const float cg = col + lane < p.N ? __ldg(p.col_scale + col + lane) : 0.f;
-            const float cu = col + lane < p.N ? __ldg(p.col_scale1 + col + lane) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; j++) {
-              v[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, cg, j));
-              u[j] = scaled((int32_t)y[j], rs, __shfl_sync(0xffffffffu, cu, j));
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; j++) {
-              v[j] = __uint_as_float(x[j]);
-              u[j] = __uint_as_float(y[j]);
-            }
-            if (p.c1) {
-              pack<O>(v, w);
-              store.put(w, &maps.c1, static_cast<O*>(p.c1), p, row0, col);
-              pack<O>(u, w);
-              store.put(w, &maps.c2, static_cast<O*>(p.c2), p, row0, col);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = gate<ACT>(v[j]) * u[j];
-        } else {
-          tmem_ld_wait();
-          if constexpr (T::I8) {
-            const float cs = col + lane < p.N ? __ldg(p.col_scale + col + lane) : 0.f;
-            const float add = p.bias && col + lane < p.N ? __ldg(p.bias + col + lane) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; j++)
-              v[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, cs, j)) + __shfl_sync(0xffffffffu, add, j);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = __uint_as_float(x[j]);
-          }
+        if constexpr (T::TWO) tmem_ld_32x32(from + (uint32_t)(128 + ch * 32), y);
+        tmem_ld_wait();
+        finish32<KIND, ACT>(p, x, y, rs, col, lane, v, g, u);
+        if (KIND == GATED && p.c1) {
+          pack<O>(g, w);
+          store.put(w, &maps.c1, static_cast<O*>(p.c1), p, row0, col);
+          pack<O>(u, w);
+          store.put(w, &maps.c2, static_cast<O*>(p.c2), p, row0, col);
         }
         pack<O>(v, w);
         if (KIND == WGRAD && z)
@@ -917,6 +923,295 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
     cluster_epilogue<KIND, O, ACT, P_THREADS, 2, PN, P_PITCH, 2>(p, tiles, split, (int)rank, z, m0, tn * CN);
     cluster_sync_all();  // shared memory stays until every CTA of the cluster has read it
   }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc2(tmem, P_TMEM_COLS);
+  }
+  if (p.wait_last) grid_dep_wait();
+}
+
+// ------------------------------------------------------------------ tall kernel
+// 512 x 256 tiles: a pair's two 256 x 256 halves share every B stage, 48 instead of 64 KiB into shared memory for the
+// same products, which is what L2 and a long run under the power cap pay for (as in tc_gemm2.cu).  The two accumulators
+// fill tensor memory, so nothing is left for the next tile: its upper half starts as soon as the upper accumulator has
+// been read, up to three k-blocks ahead of the lower, and the epilogue reads both, as packed outputs, before it stores
+// either.  Products with one weight and bf16 outputs; the gated kinds' epilogue takes too long between two tiles
+// (8192 x 8192 x 4096 with kept pre-activations 900 us here, 900 on the pair kernel; int8 4096 rows 228 and 216).
+constexpr int H_STAGES = 4;
+constexpr int H_STAGE_BYTES = 3 * A_TILE_BYTES;  // per CTA: 2 x 128 rows of A, its half of B's columns
+constexpr int H_STAGING = 4096;                  // per epilogue warp: two buffers of 32 rows x 64 bytes
+constexpr int H_CTRL = H_STAGES * H_STAGE_BYTES + P_EPI_WARPS * H_STAGING;
+constexpr int H_SMEM = H_CTRL + 1024 + 256;
+static_assert(H_SMEM <= 232448, "exceeds the shared memory a CTA can opt in to");
+
+template <int KIND>
+__global__ void __launch_bounds__(P_THREADS, 1)
+tall_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args p, int group_rows) {
+  using T = Traits<KIND>;
+  using O = __nv_bfloat16;
+  constexpr int BK = T::BK;
+  static_assert(!T::TWO, "one weight");
+  constexpr int CN = PN;
+  constexpr uint32_t IDESC = T::idesc(2 * BM, PN);
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t tiles = (raw + 1023u) & ~1023u;
+  const uint32_t bars = tiles + H_CTRL;
+  uint8_t* ctrl = smem_raw + (bars - raw);
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (H_STAGES + s); };
+  auto tfull_bar = [&](int b) { return bars + 8u * (2 * H_STAGES + b); };
+  auto tempty_bar = [&](int b) { return bars + 8u * (2 * H_STAGES + 2 + b); };
+  const uint32_t slot_addr = bars + 8u * (2 * H_STAGES + 4);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl + 8 * (2 * H_STAGES + 4));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * H_STAGES + 4) + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < H_STAGES; s++) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), 2 * P_EPI_WARPS);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 2 && lane == 0) {
+    prefetch_tensormap(&maps.a0);
+    prefetch_tensormap(&maps.b0);
+    prefetch_tensormap(&maps.c0);
+  }
+  if (warp == 1) {
+    tmem_alloc2(smem_u32(const_cast<uint32_t*>(tmem_slot)), P_TMEM_COLS);
+    tmem_relinquish2();
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  wait_before(p);
+
+  const int per_z = p.tiles_m * p.tiles_n;
+  const int num_tiles = per_z * (KIND == WGRAD ? 2 : 1);
+  const int total = p.nkb * p.segments;
+  // This pair's items: whole tiles pair, pair + num_pairs, ... of the full rounds, then one of the rest; a rest that
+  // leaves half of the pairs idle goes as half tiles (mode 1 / 2: upper / lower half alone), one a pair.
+  const int full_rounds = num_tiles / num_pairs, rest = num_tiles - full_rounds * num_pairs;
+  int last_tile = -1, last_mode = 0;
+  if (2 * rest <= num_pairs) {
+    if (pair < 2 * rest) last_tile = full_rounds * num_pairs + (pair >> 1), last_mode = 1 + (pair & 1);
+  } else if (pair < rest) {
+    last_tile = full_rounds * num_pairs + pair;
+  }
+  const int items = full_rounds + (last_tile >= 0 ? 1 : 0);
+  auto item = [&](int i, int& mode, int& z, int& tm, int& tn) {
+    const bool last = i == full_rounds;
+    int t = last ? last_tile : pair + i * num_pairs;
+    mode = last ? last_mode : 0;
+    z = t / per_z;
+    t -= z * per_z;
+    const int per_group = group_rows * p.tiles_n, group = t / per_group, first = group * group_rows;
+    const int rows = min(group_rows, p.tiles_m - first), in_group = t - group * per_group;
+    tm = first + in_group % rows;
+    tn = in_group / rows;
+  };
+  auto give_up = [&](int where) {
+    report_timeout(p.status, abort_flag, where);
+    st_cluster_u32(mapa(slot_addr + 4, rank ^ 1u), 1u);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = 0; i < items && ok; i++) {
+        int mode, z, tm, tn;
+        item(i, mode, z, tm, tn);
+        const int m0 = tm * 4 * BM + (int)rank * BM + (mode == 2 ? 2 * BM : 0);  // the lower half: + 2 BM
+        const int n0 = tn * CN + (int)rank * 128;
+        const int halves = mode ? 1 : 2;
+        for (int kb = 0; kb < total; kb++) {
+          if (!mbar_wait_relaxed(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS, 50)) {
+            give_up(81);
+            ok = false;
+            break;
+          }
+          const uint32_t bar0 = mapa(full_bar(stage), 0);
+          const uint32_t dst = tiles + stage * H_STAGE_BYTES, b_dst = dst + 2 * A_TILE_BYTES;
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * (halves + 1) * A_TILE_BYTES);
+          const bool second = kb >= p.nkb;
+          const int k0 = (second ? kb - p.nkb : kb) * BK;
+          const CUtensorMap* ma = second || (KIND == WGRAD && z) ? &maps.a1 : &maps.a0;
+          for (int h = 0; h < halves; h++) {
+            const uint32_t a_dst = dst + h * A_TILE_BYTES;
+            const int m = m0 + h * 2 * BM;
+            if (T::A_MN) {
+              for (int c = 0; c < 2; c++) tma_load_2d_pair(a_dst + c * (A_TILE_BYTES / 2), ma, bar0, m + 64 * c, k0);
+            } else {
+              tma_load_2d_pair(a_dst, ma, bar0, k0, m);
+            }
+          }
+          if (T::B_MN) {
+            const CUtensorMap* mb = second ? &maps.b1 : &maps.b0;
+            for (int c = 0; c < 2; c++) tma_load_2d_pair(b_dst + c * (A_TILE_BYTES / 2), mb, bar0, n0 + 64 * c, k0);
+          } else {
+            tma_load_2d_pair(b_dst, &maps.b0, bar0, k0, n0);
+          }
+          if (++stage == H_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok || *abort_flag) {  // error path: copies in flight land before the CTA leaves
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      // Two cursors into the ring: the upper half runs a k-block or more ahead of the lower, which frees the stages.
+      int hi_stage = 0, lo_stage = 0;
+      uint32_t hi_phase = 0, acc_phase = 0;
+      bool ok = true;
+      auto issue = [&](int stage, int half, bool first) {
+        const uint32_t a0 = tiles + stage * H_STAGE_BYTES + half * A_TILE_BYTES;
+        const uint32_t b0 = tiles + stage * H_STAGE_BYTES + 2 * A_TILE_BYTES;
+        const uint64_t da = T::A_MN ? smem_desc_mn_sw128(a0, BK) : smem_desc_k_sw128(a0);
+        const uint64_t db = T::B_MN ? smem_desc_mn_sw128(b0, BK) : smem_desc_k_sw128(b0);
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ks++)
+          tc_mma_pair<T::MMA>(tmem + (uint32_t)(half * PN), da + ks * T::step(T::A_MN), db + ks * T::step(T::B_MN), IDESC,
+                              !(first && ks == 0));
+      };
+      auto upper = [&](int kb) -> bool {
+        if (!mbar_wait(full_bar(hi_stage), hi_phase, abort_flag, WAIT_LIMIT_NS)) {
+          give_up(82);
+          return false;
+        }
+        tc_fence_after();
+        issue(hi_stage, 0, kb == 0);
+        if (++hi_stage == H_STAGES) {
+          hi_stage = 0;
+          hi_phase ^= 1u;
+        }
+        return true;
+      };
+      for (int i = 0; i < items && ok; i++) {
+        int mode, z, tm, tn;
+        item(i, mode, z, tm, tn);
+        if (!mbar_wait(tempty_bar(0), acc_phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
+          give_up(83);
+          break;
+        }
+        tc_fence_after();
+        if (mode) {  // always this pair's last item: one accumulator, stages freed at once
+          for (int kb = 0; kb < total && ok; kb++) {
+            const int stage = hi_stage;
+            ok = upper(kb);
+            if (ok) tc_commit_pair(empty_bar(stage));
+          }
+          if (ok) tc_commit_pair(tfull_bar(0));
+          break;
+        }
+        int hi = 0;  // k-blocks that the upper half has had
+        while (ok && hi < total && hi < H_STAGES - 1 && (hi < 1 || !mbar_try_wait(tempty_bar(1), acc_phase ^ 1u))) {
+          ok = upper(hi++);
+          if (ok && hi == total) tc_commit_pair(tfull_bar(0));
+        }
+        if (!ok) break;
+        if (!mbar_wait(tempty_bar(1), acc_phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
+          give_up(84);
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < total; kb++) {
+          if (hi < total && hi - kb <= 1) {
+            if (!upper(hi++)) {
+              ok = false;
+              break;
+            }
+            if (hi == total) tc_commit_pair(tfull_bar(0));
+          }
+          issue(lo_stage, 1, kb == 0);  // its stage was waited for when the upper half used it
+          tc_commit_pair(empty_bar(lo_stage));
+          if (++lo_stage == H_STAGES) lo_stage = 0;
+        }
+        if (!ok) break;
+        tc_commit_pair(tfull_bar(1));
+        acc_phase ^= 1u;
+      }
+    }
+    __syncwarp();
+  } else {
+    constexpr int BLOCKS = CN / 64;                    // 32-column blocks of this warp in a half: its half of the columns
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    BlockStore<O, H_STAGING / 2> store{tiles + H_STAGES * H_STAGE_BYTES + (uint32_t)(warp - 2) * H_STAGING, lane};
+    uint32_t acc_phase = 0;
+    // an accumulator's share of this warp as packed outputs; the accumulator goes back to the MMA thread
+    auto take = [&](int half, int row, int c0, uint32_t (&w)[BLOCKS][16]) -> bool {
+      float rs = 0.f;
+      if constexpr (T::I8)
+        if (row < p.M) rs = p.row_scale[row];
+      if (!mbar_wait_warp(tfull_bar(half), acc_phase, abort_flag, WAIT_LIMIT_NS)) {
+        if (lane == 0) give_up(85);
+        return false;
+      }
+      tc_fence_after();
+      const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * PN + part * (CN / 2));
+#pragma unroll
+      for (int b = 0; b < BLOCKS; b++) {
+        uint32_t x[32];
+        float v[32];
+        tmem_ld_32x32(from + (uint32_t)(b * 32), x);
+        tmem_ld_wait();
+        finish32<KIND, 0>(p, x, x, rs, c0 + b * 32, lane, v, v, v);
+        pack<O>(v, w[b]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa(tempty_bar(half), 0));
+      return true;
+    };
+    auto put = [&](const uint32_t (&w)[BLOCKS][16], int z, int row0, int c0) {
+      const bool second = KIND == WGRAD && z;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; b++)
+        store.put(w[b], second ? &maps.c1 : &maps.c0, static_cast<O*>(second ? p.c1 : p.c0), p, row0, c0 + b * 32);
+    };
+    for (int i = 0; i < items; i++) {
+      int mode, z, tm, tn;
+      item(i, mode, z, tm, tn);
+      const int c0 = tn * CN + part * (CN / 2);
+      const int upper0 = tm * 4 * BM + (int)rank * BM + q * 32 + (mode == 2 ? 2 * BM : 0), lower0 = upper0 + 2 * BM;
+      uint32_t upper[BLOCKS][16], lower[BLOCKS][16];
+      if (!take(0, upper0 + lane, c0, upper)) break;
+      if (mode) {
+        put(upper, z, upper0, c0);
+        break;
+      }
+      if (!take(1, lower0 + lane, c0, lower)) break;
+      put(upper, z, upper0, c0);
+      put(lower, z, lower0, c0);
+      acc_phase ^= 1u;
+    }
+    if (lane == 0) bulk_wait_all();  // shared memory outlives the stores that read it
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc2(tmem, P_TMEM_COLS);
@@ -1130,15 +1425,13 @@ cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], co
   return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a, S, stages);
 }
 
-template <int KIND, class O, int ACT, bool SPLIT>
-cudaError_t launch_pair(exo_b200_Context* ctx, const PairMaps& maps, const Args& a, int64_t tiles,
-                        bool after_own_kernel) {
-  constexpr int splits = SPLIT ? 2 : 1;
-  auto* kernel = pair_kernel<KIND, O, ACT, SPLIT>;
-  EXOB200_SMEM_ATTR_ONCE(kernel, P_SMEM, ctx->device);
+// A kernel of CTA pairs, `splits` pairs to a cluster; persistent ones on as many pairs as fit the GPU.
+template <class Kernel>
+cudaError_t launch_pairs(exo_b200_Context* ctx, Kernel* kernel, int smem, const PairMaps& maps, const Args& a,
+                         int64_t tiles, int splits, int group_rows, bool after_own_kernel) {
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(P_THREADS);
-  cfg.dynamicSmemBytes = P_SMEM;
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1146,7 +1439,7 @@ cudaError_t launch_pair(exo_b200_Context* ctx, const PairMaps& maps, const Args&
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (SPLIT) {
+  if (splits > 1) {
     cfg.gridDim = dim3(2 * (unsigned)(tiles * splits));
   } else {
     // every instance takes a whole SM, so all of them fit as many pairs; asked once per context
@@ -1165,7 +1458,35 @@ cudaError_t launch_pair(exo_b200_Context* ctx, const PairMaps& maps, const Args&
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, kernel, maps, a, 8);
+  return cudaLaunchKernelEx(&cfg, kernel, maps, a, group_rows);
+}
+
+template <int KIND, class O, int ACT, bool SPLIT>
+cudaError_t launch_pair(exo_b200_Context* ctx, const PairMaps& maps, const Args& a, int64_t tiles,
+                        bool after_own_kernel) {
+  auto* kernel = pair_kernel<KIND, O, ACT, SPLIT>;
+  EXOB200_SMEM_ATTR_ONCE(kernel, P_SMEM, ctx->device);
+  return launch_pairs(ctx, kernel, P_SMEM, maps, a, tiles, SPLIT ? 2 : 1, 8, after_own_kernel);
+}
+
+template <int KIND>
+cudaError_t launch_tall(exo_b200_Context* ctx, const PairMaps& maps, const Args& a, int64_t tiles,
+                        bool after_own_kernel) {
+  auto* kernel = tall_kernel<KIND>;
+  EXOB200_SMEM_ATTR_ONCE(kernel, H_SMEM, ctx->device);
+  return launch_pairs(ctx, kernel, H_SMEM, maps, a, tiles, 1, 6, after_own_kernel);
+}
+
+// The tall kernel where the pair kernel would run unsplit: with tiles for three pairs of four and a reduction that outlasts
+// the change from tile to tile.  Measured over 0.15 s runs, tall / pair: gradients of 8192 x 8192 x 4096 1785 / 1935 us,
+// of 4096 x 4096 x 2048 256 / 270; int8 8192^3 398 / 412, 4096^3 (32 k-blocks) 63.5 / 62.8, 4096 x 8192 x 1024 45.1 / 43.8.
+// EXOB200_FFN_TALL=0 / 1 forces it off / on.
+bool tall_wanted(const exo_b200_Context* ctx, int64_t tall_tiles, int k_blocks) {
+  static const int mode = [] {
+    const char* e = getenv("EXOB200_FFN_TALL");
+    return e ? atoi(e) : -1;
+  }();
+  return mode >= 0 ? mode == 1 : k_blocks >= 48 && tall_tiles * 8 >= 3 * ctx->sm_count;
 }
 
 // Tensor map of a dense output for 32 x 32 blocks out of swizzled shared memory
@@ -1246,6 +1567,12 @@ cudaError_t run(exo_b200_Context* ctx, const Problem& p, const Matrix& a0, const
         !(output_map<O>(&m.c0, p.c0, p.M, p.N) && (!p.c1 || output_map<O>(&m.c1, p.c1, p.M, p.N)) &&
           (!p.c2 || output_map<O>(&m.c2, p.c2, p.M, p.N))))
       return cudaErrorUnknown;
+    if constexpr (!T::TWO && sizeof(O) == 2) {
+      const int64_t tall_tiles = tiles_of(4 * BM, PN);
+      if (splits == 1 && tall_wanted(ctx, tall_tiles, a.nkb * a.segments))
+        return launch_tall<KIND>(ctx, m, a, tall_tiles, after != OTHERS);
+      tiles_of(2 * BM, PN);
+    }
     return splits > 1 ? launch_pair<KIND, O, ACT, true>(ctx, m, a, pair_tiles, after != OTHERS)
                       : launch_pair<KIND, O, ACT, false>(ctx, m, a, pair_tiles, after != OTHERS);
   }
