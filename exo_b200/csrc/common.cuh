@@ -59,7 +59,7 @@ struct exo_b200_Context {
   exob200::WeightKey wkey;
   // resident CTA pairs of the two cluster kernels on this context's device (0 = not asked yet)
   int max_pairs[4];
-  int max_ffn_pairs;  // of the feed-forward pair kernel
+  int max_ffn_pairs, max_ffn_split;  // the same for the feed-forward kernels; largest cluster of their split kernel
   exob200::DeviceStatus* status_dev;   // device word
   exob200::DeviceStatus* status_host;  // pinned mirror
   // host-pointer row pipeline: copy-in / copy-out streams, two chunk buffers each way

@@ -12,6 +12,20 @@ bool refuse(const char* fn, bool cond, const std::string& what, int code = EXO_B
   return cond;
 }
 
+// Nothing is thrown through a C entry (a failing allocation of a message, a mutex): it becomes the call's error.
+template <class F>
+void guarded(const char* fn, F body) {
+  try {
+    clear_error();
+    body();
+  } catch (...) {
+    try {
+      set_error(EXO_B200_ERR_CUDA, std::string(fn) + ": host-side failure");
+    } catch (...) {
+    }
+  }
+}
+
 // sums of K products of int8 fit int32 up to here: 131071 * 128 * 128 < 2^31
 constexpr int_fast32_t kMaxI8K = 131071;
 
@@ -129,7 +143,6 @@ size_t mul(int_fast32_t a, int_fast32_t b, size_t e) { return (size_t)a * (size_
 
 void quantize(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t K, const void* X, bool bf16, int8_t* Q,
               float* scale) {
-  clear_error();
   if (bad_sizes(fn, M, K, 1, "M and K")) return;
   const size_t e = bf16 ? 2 : 4;
   Operands o(fn, ctxt);
@@ -140,7 +153,6 @@ void quantize(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t K, const 
 void gemm_scaled(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const int8_t* A,
                  const int8_t* B, const float* row_scale, const float* col_scale, const float* bias, void* C,
                  bool f32) {
-  clear_error();
   if (bad_sizes(fn, M, N, K, "M, N, K")) return;
   if (refuse(fn, K > kMaxI8K, "K above 131071 would overflow the int32 sums", EXO_B200_ERR_UNSUPPORTED)) return;
   const size_t e = f32 ? 4 : 2;
@@ -164,7 +176,6 @@ void gemm_scaled(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t N, int
 void linear(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const void* X,
             const int8_t* B, const float* col_scale, const float* bias, int8_t* Q, float* row_scale, void* Y,
             bool f32) {
-  clear_error();
   if (bad_sizes(fn, M, N, K, "M, N, K")) return;
   if (refuse(fn, K > kMaxI8K, "K above 131071 would overflow the int32 sums", EXO_B200_ERR_UNSUPPORTED)) return;
   const size_t e = f32 ? 4 : 2;
@@ -193,41 +204,9 @@ void linear(const char* fn, void* ctxt, int_fast32_t M, int_fast32_t N, int_fast
   o.done(err);
 }
 
-}  // namespace
-
-extern "C" {
-
-void quantize_rows_bf16_exo(void* ctxt, int_fast32_t M, int_fast32_t K, const uint16_t* X, int8_t* Q, float* scale) {
-  quantize("quantize_rows_bf16_exo", ctxt, M, K, X, true, Q, scale);
-}
-void quantize_rows_f32_exo(void* ctxt, int_fast32_t M, int_fast32_t K, const float* X, int8_t* Q, float* scale) {
-  quantize("quantize_rows_f32_exo", ctxt, M, K, X, false, Q, scale);
-}
-
-void gemm_i8_scaled_bf16_exo(void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const int8_t* A,
-                             const int8_t* B, const float* row_scale, const float* col_scale, const float* bias,
-                             uint16_t* C) {
-  gemm_scaled("gemm_i8_scaled_bf16_exo", ctxt, M, N, K, A, B, row_scale, col_scale, bias, C, false);
-}
-void gemm_i8_scaled_f32_exo(void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const int8_t* A,
-                            const int8_t* B, const float* row_scale, const float* col_scale, const float* bias,
-                            float* C) {
-  gemm_scaled("gemm_i8_scaled_f32_exo", ctxt, M, N, K, A, B, row_scale, col_scale, bias, C, true);
-}
-
-void linear_i8_bf16_exo(void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const uint16_t* X, const int8_t* B,
-                        const float* col_scale, const float* bias, int8_t* Q, float* row_scale, uint16_t* Y) {
-  linear("linear_i8_bf16_exo", ctxt, M, N, K, X, B, col_scale, bias, Q, row_scale, Y, false);
-}
-void linear_i8_f32_exo(void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const float* X, const int8_t* B,
-                       const float* col_scale, const float* bias, int8_t* Q, float* row_scale, float* Y) {
-  linear("linear_i8_f32_exo", ctxt, M, N, K, X, B, col_scale, bias, Q, row_scale, Y, true);
-}
-
-void gated_bf16_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
+void gated(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
                     const uint16_t* X, const uint16_t* Wg, const uint16_t* Wu, uint16_t* H, uint16_t* G, uint16_t* U) {
   const char* fn = "gated_bf16_exo";
-  clear_error();
   if (bad_act(fn, activation) || bad_sizes(fn, M, F, K, "M, F, K")) return;
   if (refuse(fn, !G != !U, "G and U are kept together: give both or neither")) return;
   Operands o(fn, ctxt);
@@ -247,12 +226,11 @@ void gated_bf16_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fas
   o.done(ffn::launch_product(o.ctx(), ffn::GATED, false, p, false));
 }
 
-void gated_bf16_backward_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
+void gated_backward(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
                              const uint16_t* X, const uint16_t* Wg, const uint16_t* Wu, const uint16_t* G,
                              const uint16_t* U, const uint16_t* dH, uint16_t* dG, uint16_t* dU, uint16_t* dX,
                              uint16_t* dWg, uint16_t* dWu) {
   const char* fn = "gated_bf16_backward_exo";
-  clear_error();
   if (bad_act(fn, activation) || bad_sizes(fn, M, F, K, "M, F, K")) return;
   if (refuse(fn, !dWg != !dWu, "dWg and dWu are computed together: give both or neither")) return;
   Operands o(fn, ctxt);
@@ -277,11 +255,10 @@ void gated_bf16_backward_exo(void* ctxt, int_fast32_t activation, int_fast32_t M
   o.done(e);
 }
 
-void gated_i8_bf16_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
+void gated_i8(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
                        const int8_t* A, const int8_t* Bg, const int8_t* Bu, const float* row_scale,
                        const float* gate_scale, const float* up_scale, uint16_t* H) {
   const char* fn = "gated_i8_bf16_exo";
-  clear_error();
   if (bad_act(fn, activation) || bad_sizes(fn, M, F, K, "M, F, K")) return;
   if (refuse(fn, K > kMaxI8K, "K above 131071 would overflow the int32 sums", EXO_B200_ERR_UNSUPPORTED)) return;
   Operands o(fn, ctxt);
@@ -301,6 +278,65 @@ void gated_i8_bf16_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_
   p.c0 = o.dev<void>(6);
   p.act = (int)activation;
   o.done(ffn::launch_product(o.ctx(), ffn::GATED_I8, false, p, false));
+}
+
+}  // namespace
+
+extern "C" {
+
+void quantize_rows_bf16_exo(void* ctxt, int_fast32_t M, int_fast32_t K, const uint16_t* X, int8_t* Q, float* scale) {
+  guarded("quantize_rows_bf16_exo", [&] { quantize("quantize_rows_bf16_exo", ctxt, M, K, X, true, Q, scale); });
+}
+void quantize_rows_f32_exo(void* ctxt, int_fast32_t M, int_fast32_t K, const float* X, int8_t* Q, float* scale) {
+  guarded("quantize_rows_f32_exo", [&] { quantize("quantize_rows_f32_exo", ctxt, M, K, X, false, Q, scale); });
+}
+
+void gemm_i8_scaled_bf16_exo(void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const int8_t* A,
+                             const int8_t* B, const float* row_scale, const float* col_scale, const float* bias,
+                             uint16_t* C) {
+  guarded("gemm_i8_scaled_bf16_exo", [&] {
+    gemm_scaled("gemm_i8_scaled_bf16_exo", ctxt, M, N, K, A, B, row_scale, col_scale, bias, C, false);
+  });
+}
+void gemm_i8_scaled_f32_exo(void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const int8_t* A,
+                            const int8_t* B, const float* row_scale, const float* col_scale, const float* bias,
+                            float* C) {
+  guarded("gemm_i8_scaled_f32_exo", [&] {
+    gemm_scaled("gemm_i8_scaled_f32_exo", ctxt, M, N, K, A, B, row_scale, col_scale, bias, C, true);
+  });
+}
+
+void linear_i8_bf16_exo(void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const uint16_t* X, const int8_t* B,
+                        const float* col_scale, const float* bias, int8_t* Q, float* row_scale, uint16_t* Y) {
+  guarded("linear_i8_bf16_exo", [&] {
+    linear("linear_i8_bf16_exo", ctxt, M, N, K, X, B, col_scale, bias, Q, row_scale, Y, false);
+  });
+}
+void linear_i8_f32_exo(void* ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const float* X, const int8_t* B,
+                       const float* col_scale, const float* bias, int8_t* Q, float* row_scale, float* Y) {
+  guarded("linear_i8_f32_exo", [&] {
+    linear("linear_i8_f32_exo", ctxt, M, N, K, X, B, col_scale, bias, Q, row_scale, Y, true);
+  });
+}
+
+void gated_bf16_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
+                    const uint16_t* X, const uint16_t* Wg, const uint16_t* Wu, uint16_t* H, uint16_t* G, uint16_t* U) {
+  guarded("gated_bf16_exo", [&] { gated(ctxt, activation, M, F, K, X, Wg, Wu, H, G, U); });
+}
+
+void gated_bf16_backward_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
+                             const uint16_t* X, const uint16_t* Wg, const uint16_t* Wu, const uint16_t* G,
+                             const uint16_t* U, const uint16_t* dH, uint16_t* dG, uint16_t* dU, uint16_t* dX,
+                             uint16_t* dWg, uint16_t* dWu) {
+  guarded("gated_bf16_backward_exo",
+          [&] { gated_backward(ctxt, activation, M, F, K, X, Wg, Wu, G, U, dH, dG, dU, dX, dWg, dWu); });
+}
+
+void gated_i8_bf16_exo(void* ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K,
+                       const int8_t* A, const int8_t* Bg, const int8_t* Bu, const float* row_scale,
+                       const float* gate_scale, const float* up_scale, uint16_t* H) {
+  guarded("gated_i8_bf16_exo",
+          [&] { gated_i8(ctxt, activation, M, F, K, A, Bg, Bu, row_scale, gate_scale, up_scale, H); });
 }
 
 }  // extern "C"

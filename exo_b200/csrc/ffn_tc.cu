@@ -15,6 +15,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdlib>
 
 #include "ffn.cuh"
@@ -1333,15 +1334,55 @@ bool map_of(CUtensorMap* m, const Matrix& x, int elem, int box_rows) {
                           dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+#define EXOB200_CLUSTER16_ONCE(kernel, device)                                                                        \
+  do {                                                                                                                \
+    static std::atomic<uint64_t> done_{0};                                                                            \
+    const uint64_t bit_ = 1ull << ((device) & 63);                                                                    \
+    if (!(done_.load(std::memory_order_acquire) & bit_)) {                                                            \
+      cudaError_t e_ = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);               \
+      if (e_ != cudaSuccess) return e_;                                                                               \
+      done_.fetch_or(bit_, std::memory_order_release);                                                                \
+    }                                                                                                                 \
+  } while (0)
+
+// The largest cluster of the split kernel: MAX_SPLIT where the GPU has room for one (asked once per context, of one
+// instance: all of them take their SM), else eight.
+cudaError_t ask_max_split(exo_b200_Context* ctx, int* most) {
+  auto* kernel = split_kernel<DGRAD, __nv_bfloat16, 0, false>;
+  EXOB200_SMEM_ATTR_ONCE(kernel, S_SMEM_ALONE, ctx->device);
+  EXOB200_CLUSTER16_ONCE(kernel, ctx->device);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(MAX_SPLIT);
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = S_SMEM_ALONE;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = MAX_SPLIT;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  if (e == cudaSuccess) *most = n >= 4 ? MAX_SPLIT : 8;
+  return e;
+}
+int max_split(exo_b200_Context* ctx) {
+  if (ctx->max_ffn_split == 0 && ask_max_split(ctx, &ctx->max_ffn_split) != cudaSuccess) {
+    cudaGetLastError();
+    ctx->max_ffn_split = 8;
+  }
+  return ctx->max_ffn_split;
+}
+
 // How many CTAs of the split kernel share a tile's reduction: as long as every CTA has an SM to itself and two k-blocks.
 // (256 x 2048 x 4096 int8, 32 tiles: 14.3, 10.5, 9.5 and 14.8 us with 1, 2, 4 and 8 CTAs a tile; 512 x 2048 x 4096, 64
 // tiles: 14.7, 11.0, 13.0 and 26.7: past one CTA for each SM, and mostly past four of them on one tile, adding up costs
 // more than the shorter loops save.)  A handful of tiles with a long reduction splits further (the gradient of 3 x 177
-// inputs over 2 x 14054 units, two tiles: FILL_S4 us with four, 12.8 with sixteen).
-int split_of(const exo_b200_Context* ctx, int64_t tiles, int k_blocks) {
+// inputs over 2 x 14054 units, two tiles: 33 us of a 60 us backward pass with four, 12.8 with sixteen).
+int split_of(exo_b200_Context* ctx, int64_t tiles, int k_blocks) {
   int S = 1;
   while (S < 4 && tiles * S * 2 <= ctx->sm_count && k_blocks / (2 * S) >= 2) S *= 2;
-  while (S >= 4 && S < MAX_SPLIT && tiles * S * 4 <= ctx->sm_count && k_blocks / (2 * S) >= 8) S *= 2;
+  while (S >= 4 && S < max_split(ctx) && tiles * S * 4 <= ctx->sm_count && k_blocks / (2 * S) >= 8) S *= 2;
   return S;
 }
 
@@ -1353,7 +1394,7 @@ int split_of(const exo_b200_Context* ctx, int64_t tiles, int k_blocks) {
 // of tiles the time is a fixed part and so much for each k-block that one CTA goes through: fitted, in us, on products
 // and gated products of 160 to 2048 rows, 512 to 8192 columns and 2 to 64 k-blocks (split / pair / two pairs measured:
 // 1024 x 1024 x 1024 int8 7.6 / 9.5 / 9.3, 1024 x 4096 x 4096 19.9 / 19.1 / 28, 512 x 4096 x 4096 15.9 / 17.0 / 14.0).
-int pair_splits(const exo_b200_Context* ctx, int64_t rows, int64_t pair_tiles, int64_t split_tiles, int k_blocks) {
+int pair_splits(exo_b200_Context* ctx, int64_t rows, int64_t pair_tiles, int64_t split_tiles, int k_blocks) {
   static const int mode = [] {
     const char* e = getenv("EXOB200_FFN_PAIR");
     return e ? atoi(e) : -1;
@@ -1390,15 +1431,7 @@ cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], co
   const int total = a.nkb * a.segments;
   const int S = split_of(ctx, tiles, total);
   if (tiles * S > INT32_MAX) return cudaErrorInvalidValue;
-  if (S > 8) {
-    static std::atomic<uint64_t> allowed{0};
-    const uint64_t bit = 1ull << (ctx->device & 63);
-    if (!(allowed.load(std::memory_order_acquire) & bit)) {
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return e;
-      allowed.fetch_or(bit, std::memory_order_release);
-    }
-  }
+  if (S > 8) EXOB200_CLUSTER16_ONCE(kernel, ctx->device);
   const int stage_bytes = (Traits<KIND>::A_MN ? A_TILE_BYTES : a.a_rows * ROW_BYTES) + A_TILE_BYTES;
   const int room = (tiles * S <= ctx->sm_count ? S_SMEM_ALONE : S_SMEM_SHARED) - S_CTRL;
   const int stages = std::min(S_MAX_STAGES, room / stage_bytes);
@@ -1415,7 +1448,7 @@ cudaError_t launch_split(exo_b200_Context* ctx, const CUtensorMap (&maps)[4], co
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     n++;
   }
-  if (after_own_kernel) {
+  if (after_own_kernel && dependent_launches()) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n].val.programmaticStreamSerializationAllowed = 1;
     n++;
@@ -1453,7 +1486,7 @@ cudaError_t launch_pairs(exo_b200_Context* ctx, Kernel* kernel, int smem, const 
     }
     cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, max_pairs));
   }
-  if (after_own_kernel) {
+  if (after_own_kernel && dependent_launches()) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;

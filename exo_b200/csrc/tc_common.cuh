@@ -144,13 +144,16 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Launches `kernel` so that it may begin before the preceding kernel of the stream has finished (the
 // kernel calls grid_dep_wait() before it touches that kernel's output).  EXOB200_PDL=0 turns the
 // attribute off (plain stream order).
-template <class... KArgs, class... Args>
-cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                             Args&&... args) {
-  static const bool pdl = [] {
+inline bool dependent_launches() {
+  static const bool on = [] {
     const char* e = getenv("EXOB200_PDL");
     return !(e && e[0] == '0');
   }();
+  return on;
+}
+template <class... KArgs, class... Args>
+cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                             Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -160,7 +163,7 @@ cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = dependent_launches() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 

@@ -1,5 +1,9 @@
 """Feed-forward operators: int8 products with token and channel scales, gated projections, their backward pass.
 Plain float64 oracle in tests/ffn_oracle.py; the bounds are derived there."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -680,3 +684,141 @@ def test_entry_points_of_both_wrappers_agree_on_the_stream(lib):
             s.synchronize()
             want.setdefault("y", float(got))
             assert float(got) == want["y"] != 0.0
+
+
+# ------------------------------------------------------------------ sizes of the large kernels, oracle on the GPU in float64
+def gpu_close(got, want, bound):
+    import torch
+
+    bad = ~((got.double() - want).abs() <= bound)
+    assert not bool(bad.any()), (int(bad.sum()), got[bad][:4], want[bad][:4])
+
+
+def gpu_normal(seed, *shape, std=1.0):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * std).bfloat16()
+
+
+def gpu_int8(seed, rows, k):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randint(-127, 128, (rows, k), generator=g, device="cuda", dtype=torch.int8),
+            torch.rand(rows, generator=g, device="cuda") * 0.02 + 0.001)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,kind", [(4096, 4096, 8192, "bf16"), (4100, 3990, 8208, "bf16"), (4099, 4001, 8191, "bf16"),
+                                        (3000, 2600, 6400, "f32"), (512, 4096, 4096, "bf16"), (520, 4000, 4000, "f32"),
+                                        (300, 700, 20000, "bf16"), (20, 100, 65536, "f32")])
+def test_gemm_i8_scaled_large(lib, M, N, K, kind):
+    import torch
+
+    (a, row), (b, col) = gpu_int8(1, M, K), gpu_int8(2, N, K)
+    bias = torch.randn(N, device="cuda")
+    c = torch.empty(M, N, dtype=torch.bfloat16 if kind == "bf16" else torch.float32, device="cuda")
+    getattr(lib, f"gemm_i8_scaled_{kind}_exo")(None, M, N, K, a, b, row, col, bias, c)
+    s = a.double() @ b.double().T * row.double()[:, None] * col.double()
+    want = s + bias.double()
+    bound = 4 * fo.U32 * (s.abs() + want.abs())
+    gpu_close(c, want, bound if kind == "f32" else bound * (1 + fo.U16) + fo.U16 * want.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,F,K", [(4096, 4096, 2048), (4100, 4104, 1000), (3500, 4097, 2001), (5, 9000, 200), (4200, 300, 260)])
+def test_gated_backward_large(lib, M, F, K):
+    """The bounds of backward_oracle, with the products of magnitudes on the GPU."""
+    import torch
+
+    x, wg, wu = gpu_normal(1, M, K), gpu_normal(2, F, K, std=0.02), gpu_normal(3, F, K, std=0.02)
+    g, u, dh = gpu_normal(4, M, F), gpu_normal(5, M, F), gpu_normal(6, M, F, std=0.01)
+    e = lambda *s: torch.empty(s, dtype=torch.bfloat16, device="cuda")
+    dg, du, dx, dwg, dwu = e(M, F), e(M, F), e(M, K), e(F, K), e(F, K)
+    lib.gated_bf16_backward_exo(None, fo.SILU, M, F, K, x, wg, wu, g, u, dh, dg, du, dx, dwg, dwu)
+    g, u, dh, x, wg, wu = (t.double() for t in (g, u, dh, x, wg, wu))
+    p = torch.sigmoid(g)
+    a, slope = g * p, p + g * p * (1 - p)
+    wdg, wdu = dh * u * slope, dh * a
+    half = lambda y, err: err * (1 + fo.U16) + fo.U16 * y.abs() + fo.TINY16
+    eg = half(wdg, (dh * u).abs() * 2.0 ** -18 * (1 + slope.abs()))
+    eu = half(wdu, dh.abs() * (2.0 ** -19 * a.abs() + 2.0 ** -20 * g.abs().clamp_max(1)))
+    gpu_close(dg, wdg, eg)
+    gpu_close(du, wdu, eu)
+    mg, mu = wdg.abs() + eg, wdu.abs() + eu
+    want = wdg @ wg + wdu @ wu
+    gpu_close(dx, want, half(want, eg @ wg.abs() + eu @ wu.abs() + fo.sum_slack(2 * F) * (mg @ wg.abs() + mu @ wu.abs())))
+    for got, d, ed, md in ((dwg, wdg, eg, mg), (dwu, wdu, eu, mu)):
+        want = d.T @ x
+        gpu_close(got, want, half(want, ed.T @ x.abs() + fo.sum_slack(M) * (md.T @ x.abs())))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,F,K", [(4096, 4096, 1024), (4099, 4103, 520), (1024, 1024, 4096), (1, 16384, 4095), (20, 6000, 3001)])
+def test_gated_large(lib, M, F, K):
+    import torch
+
+    x, wg, wu = gpu_normal(1, M, K), gpu_normal(2, F, K, std=0.02), gpu_normal(3, F, K, std=0.02)
+    h, g, u = (torch.empty(M, F, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    lib.gated_bf16_exo(None, fo.SILU, M, F, K, x, wg, wu, h, g, u)
+    x, wg, wu = (t.double() for t in (x, wg, wu))
+    wantg, wantu = x @ wg.T, x @ wu.T
+    eg, eu = (fo.sum_slack(K) * (x.abs() @ w.abs().T) for w in (wg, wu))
+    half = lambda y, err: err * (1 + fo.U16) + fo.U16 * y.abs() + fo.TINY16
+    gpu_close(g, wantg, half(wantg, eg))
+    gpu_close(u, wantu, half(wantu, eu))
+    a = wantg * torch.sigmoid(wantg)
+    ea = 1.2 * eg + 2.0 ** -19 * a.abs() + 2.0 ** -20 * wantg.abs().clamp_max(1)
+    want = a * wantu
+    gpu_close(h, want, half(want, ea * wantu.abs() + a.abs() * eu + ea * eu + 2 * fo.U32 * want.abs()))
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(lib):
+    """More than 2^31 elements in an output, an input and a weight; rows at both ends and around the border."""
+    import torch
+
+    M, N, K = 70000, 33000, 16
+    (a, row), (b, col) = gpu_int8(1, M, K), gpu_int8(2, N, K)
+    c = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    lib.gemm_i8_scaled_bf16_exo(None, M, N, K, a, b, row, col, None, c)
+    rows = torch.tensor([0, 1, 2 ** 31 // N - 1, 2 ** 31 // N, 2 ** 31 // N + 1, M - 1], device="cuda")
+    s = a[rows].double() @ b.double().T * row[rows].double()[:, None] * col.double()
+    gpu_close(c[rows], s, 8 * fo.U32 * s.abs() * 2 + fo.U16 * s.abs())
+    del c
+    M, K = 40000, 60000  # X and Q
+    x = torch.empty(M, K, dtype=torch.bfloat16, device="cuda").normal_()
+    q, s = torch.empty(M, K, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    lib.quantize_rows_bf16_exo(None, M, K, x, q, s)
+    rows = [0, 2 ** 31 // K, 2 ** 31 // K + 1, M - 1]
+    want_q, want_s = fo.quantize_rows(x[rows].float().cpu().numpy())
+    assert np.array_equal(q[rows].cpu().numpy(), want_q) and np.array_equal(s[rows].cpu().numpy(), want_s)
+    del x
+    # Q as the weight of a few tokens: the last channels lie beyond 2^31
+    for m in (2, 24):
+        t, ts = gpu_int8(5, m, K)
+        y = torch.empty(m, M, device="cuda")
+        lib.gemm_i8_scaled_f32_exo(None, m, M, K, t, q, ts, s, None, y)
+        want = t.double() @ q[rows].double().T * ts.double()[:, None] * s[rows].double()
+        gpu_close(y[:, rows], want, 8 * fo.U32 * want.abs() * 2)
+
+
+VARIANTS = {
+    "split kernel": {"EXOB200_FFN_PAIR": "0", "EXOB200_FFN_ROWS": "0"},
+    "pairs": {"EXOB200_FFN_PAIR": "1", "EXOB200_FFN_TALL": "0", "EXOB200_FFN_ROWS": "0"},
+    "tall tiles": {"EXOB200_FFN_PAIR": "1", "EXOB200_FFN_TALL": "1", "EXOB200_FFN_ROWS": "0"},
+    "two pairs a tile": {"EXOB200_FFN_PAIR": "2", "EXOB200_FFN_ROWS": "0"},
+    "copied operands, plain launches": {"EXOB200_FFN_GATHER": "0", "EXOB200_FFN_ROWS": "0", "EXOB200_PDL": "0"},
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", VARIANTS)
+def test_every_kernel_at_every_size(variant):
+    """The sizes above with each kernel forced (in a process of its own: the switches are read once)."""
+    names = "test_gemm_i8_scaled or test_linear or test_gated or unaligned or captured or block"
+    r = subprocess.run([sys.executable, "-m", "pytest", __file__, "-x", "-q", "-m", "gpu", "-k",
+                        f"({names}) and not large and not every_kernel"], capture_output=True, text=True,
+                       env={**os.environ, **VARIANTS[variant]}, timeout=600)
+    assert r.returncode == 0 and " passed" in r.stdout, r.stdout[-3000:] + r.stderr[-2000:]
