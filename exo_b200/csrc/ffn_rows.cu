@@ -11,7 +11,7 @@ using tc::aligned16;
 using umma::grid_dep_launch;
 
 // ------------------------------------------------------------------ quantisation
-// Largest of the magnitudes over the WARPS warps that share a row.
+// Largest of the magnitudes over the warp, or the CTA's eight warps, that share a row.
 template <int WARPS>
 __device__ __forceinline__ unsigned row_top(unsigned top) {
   top = __reduce_max_sync(0xffffffffu, top);
@@ -26,15 +26,16 @@ __device__ __forceinline__ unsigned row_top(unsigned top) {
 }
 
 // Rows that are whole 16-byte vectors: each is read once and stays in registers (V vectors a thread) between the search
-// for its largest magnitude and the rounding.  A CTA takes one row (WARPS = 8) or, where a row is short, a warp does.
-// 2048 x 4096 bf16: 7.3 us, 10.0 with the two passes below.
+// for its largest magnitude and the rounding.  Where rows are many and short, a warp takes one, with up to eight loads in
+// flight and no one to agree with (8192 x 1024 fp32: 6.6 us, 10.8 with a CTA a row); otherwise a CTA (2048 x 4096 bf16:
+// 4.8 us, 4.9 with two warps a row; 8192 x 8192 33 us, 6.1 TB/s, 38 with four).
 template <class E, int V, int WARPS>
 __global__ void __launch_bounds__(256) quantize_vectors_kernel(int64_t M, int K, const E* X, int8_t* Q, float* scale) {
   constexpr int N = 16 / sizeof(E);
   grid_dep_launch();
-  const int64_t row = (int64_t)blockIdx.x * (8 / WARPS) + (WARPS == 8 ? 0 : threadIdx.x / 32);
+  const int64_t row = (int64_t)blockIdx.x * (8 / WARPS) + threadIdx.x / (32 * WARPS);
+  if (row >= M) return;
   const int t = threadIdx.x % (32 * WARPS);
-  if (WARPS == 1 && row >= M) return;
   const uint4* x = reinterpret_cast<const uint4*>(X + row * K);
   uint4 v[V];
   unsigned top = 0;
@@ -73,9 +74,9 @@ __global__ void __launch_bounds__(256) quantize_vectors_kernel(int64_t M, int K,
 template <class E, int WARPS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t M, int64_t K, const E* X, int8_t* Q, float* scale) {
   grid_dep_launch();
-  const int64_t row = (int64_t)blockIdx.x * (8 / WARPS) + (WARPS == 8 ? 0 : threadIdx.x / 32);
+  const int64_t row = (int64_t)blockIdx.x * (8 / WARPS) + threadIdx.x / (32 * WARPS);
+  if (row >= M) return;  // a warp's, or none: a CTA that shares a row has one
   const int t = threadIdx.x % (32 * WARPS);
-  if (WARPS == 1 && row >= M) return;
   const E* x = X + row * K;
   int8_t* q = Q + row * K;
   unsigned top = 0;
@@ -93,9 +94,11 @@ cudaError_t quantize(exo_b200_Context* ctx, int64_t M, int64_t K, const E* X, in
   const cudaStream_t st = ctx->stream;
   const bool vectors = K % N == 0 && aligned16(X) && reinterpret_cast<uintptr_t>(Q) % N == 0;
   const unsigned m = (unsigned)M;
-  // a warp a row where that leaves no thread idle for want of columns and there are rows for every SM
-  if (vectors && K <= 128 * N && M >= 8 * ctx->sm_count)
+  const bool many = M >= 8 * ctx->sm_count;
+  if (vectors && many && K <= 128 * N)
     quantize_vectors_kernel<E, 4, 1><<<(m + 7) / 8, 256, 0, st>>>(M, (int)K, X, Q, scale);
+  else if (vectors && many && K <= 256 * N)
+    quantize_vectors_kernel<E, 8, 1><<<(m + 7) / 8, 256, 0, st>>>(M, (int)K, X, Q, scale);
   else if (vectors && K <= 256 * N)
     quantize_vectors_kernel<E, 1, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
   else if (vectors && K <= 512 * N)
@@ -104,6 +107,8 @@ cudaError_t quantize(exo_b200_Context* ctx, int64_t M, int64_t K, const E* X, in
     quantize_vectors_kernel<E, 4, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
   else if (vectors && K <= 2048 * N)
     quantize_vectors_kernel<E, 8, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
+  else if (vectors && K <= 4096 * N)
+    quantize_vectors_kernel<E, 16, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
   else if (K <= 1024 && M >= 8 * ctx->sm_count)
     quantize_rows_kernel<E, 1><<<(m + 7) / 8, 256, 0, st>>>(M, K, X, Q, scale);
   else

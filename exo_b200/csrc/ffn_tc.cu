@@ -560,7 +560,7 @@ constexpr int P_STAGES = 5;                       // six let the pairs drift apa
 constexpr int P_STAGE_BYTES = 2 * A_TILE_BYTES;   // per CTA: 128 rows of A, its half (128) of B's columns
 constexpr int P_EPI_WARPS = 8;                    // two for each tensor-memory lane quarter, half the columns each
 constexpr int P_THREADS = 32 * (2 + P_EPI_WARPS);
-constexpr int P_STAGING = 8192;                   // per epilogue warp: two buffers of 32 rows x 128 bytes
+constexpr int P_STAGING = 8192;                   // per epilogue warp: 32-row blocks, two of fp32 or four of bf16
 constexpr int P_CTRL = P_STAGES * P_STAGE_BYTES + P_EPI_WARPS * P_STAGING;
 constexpr int P_SMEM = P_CTRL + 1024 + 256;
 static_assert(P_SMEM <= 232448, "exceeds the shared memory a CTA can opt in to");
@@ -577,19 +577,20 @@ struct PairMaps {
 // With a map for C: whole rows go out through the copy engine, which clips at C's edges; shared memory is
 // swizzled so that the 128-bit writes meet no bank twice.  Without (a pitch or base that TMA cannot take): rows leave
 // one by one, lane = column.
-template <class O, int BUFFER>
+template <class O, int AREA>
 struct BlockStore {
   static constexpr int WORDS = sizeof(O) == 2 ? 16 : 32;
-  uint32_t area;  // this warp's staging: two buffers
+  static constexpr int BUFFERS = AREA / (32 * WORDS * 4);
+  uint32_t area;  // this warp's staging
   int lane, buf = 0;
 
   __device__ __forceinline__ void put(const uint32_t (&w)[WORDS], const CUtensorMap* m, O* C, const Args& p, int row0,
                                       int col) {
     if (row0 >= p.M || col >= p.N) return;
     if (p.vec) {
-      if (lane == 0) bulk_wait_read_1();  // the store that last used this buffer has read it
+      if (lane == 0) bulk_wait_read<BUFFERS - 1>();  // the store that last used this buffer has read it
       __syncwarp();
-      const uint32_t at = area + (uint32_t)(buf * BUFFER);
+      const uint32_t at = area + (uint32_t)(buf * 32 * WORDS * 4);
 #pragma unroll
       for (int j = 0; j < WORDS / 4; j++) {
         const int swizzled = sizeof(O) == 2 ? j ^ ((lane >> 1) & 3) : j ^ (lane & 7);
@@ -604,7 +605,7 @@ struct BlockStore {
         tma_store_2d(m, at, col, row0);
         bulk_commit();
       }
-      buf ^= 1;
+      buf = (buf + 1) % BUFFERS;
     } else {
       __syncwarp();
 #pragma unroll
@@ -867,7 +868,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
     }
   } else {
     const int q = warp & 3, part = (warp - 2) >> 2;
-    BlockStore<O, P_STAGING / 2> store{tiles + P_STAGES * P_STAGE_BYTES + (uint32_t)(warp - 2) * P_STAGING, lane};
+    BlockStore<O, P_STAGING> store{tiles + P_STAGES * P_STAGE_BYTES + (uint32_t)(warp - 2) * P_STAGING, lane};
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = pair; t < num_tiles; t += num_pairs) {
@@ -887,7 +888,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
 #pragma unroll 1
       for (int ch = 0; ch < CN / 64; ch++) {
         const int col = c0 + ch * 32;
-        uint32_t x[32], y[32], w[BlockStore<O, P_STAGING / 2>::WORDS];
+        uint32_t x[32], y[32], w[BlockStore<O, P_STAGING>::WORDS];
         float v[32], g[32], u[32];
         tmem_ld_32x32(from + (uint32_t)(ch * 32), x);
         if constexpr (T::TWO) tmem_ld_32x32(from + (uint32_t)(128 + ch * 32), y);
@@ -940,7 +941,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
 // (8192 x 8192 x 4096 with kept pre-activations 900 us here, 900 on the pair kernel; int8 4096 rows 228 and 216).
 constexpr int H_STAGES = 4;
 constexpr int H_STAGE_BYTES = 3 * A_TILE_BYTES;  // per CTA: 2 x 128 rows of A, its half of B's columns
-constexpr int H_STAGING = 4096;                  // per epilogue warp: two buffers of 32 rows x 64 bytes
+constexpr int H_STAGING = 4096;                  // per epilogue warp: two 32-row blocks of bf16
 constexpr int H_CTRL = H_STAGES * H_STAGE_BYTES + P_EPI_WARPS * H_STAGING;
 constexpr int H_SMEM = H_CTRL + 1024 + 256;
 static_assert(H_SMEM <= 232448, "exceeds the shared memory a CTA can opt in to");
@@ -1158,7 +1159,7 @@ tall_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
   } else {
     constexpr int BLOCKS = CN / 64;                    // 32-column blocks of this warp in a half: its half of the columns
     const int q = warp & 3, part = (warp - 2) >> 2;
-    BlockStore<O, H_STAGING / 2> store{tiles + H_STAGES * H_STAGE_BYTES + (uint32_t)(warp - 2) * H_STAGING, lane};
+    BlockStore<O, H_STAGING> store{tiles + H_STAGES * H_STAGE_BYTES + (uint32_t)(warp - 2) * H_STAGING, lane};
     uint32_t acc_phase = 0;
     // an accumulator's share of this warp as packed outputs; the accumulator goes back to the MMA thread
     auto take = [&](int half, int row, int c0, uint32_t (&w)[BLOCKS][16]) -> bool {

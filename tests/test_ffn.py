@@ -179,7 +179,8 @@ def values(g):
     return widen(a.view(np.uint16)) if a.dtype == np.int16 else a
 
 
-QUANT_SHAPES = [(1, 1), (1, 4096), (3, 7), (5, 33), (130, 1000), (7, 4099), (2, 40000), (300, 128), (4, 16384)]
+QUANT_SHAPES = [(1, 1), (1, 4096), (3, 7), (5, 33), (130, 1000), (7, 4099), (2, 40000), (300, 128), (4, 16384), (5, 8200),
+                (3, 32768), (1300, 512), (1301, 1000), (1200, 2040), (1250, 77), (3, 2056)]
 
 
 @pytest.mark.gpu
