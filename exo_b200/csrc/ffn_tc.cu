@@ -646,21 +646,38 @@ __device__ __forceinline__ void pack(const float (&v)[32], uint32_t (&w)[W]) {
   }
 }
 
-// 32 columns (from col) of one accumulator row: sums x, of the up projection y, to output values v; gated products leave
-// their pre-activations in g and u.
+// What a warp's BLOCKS blocks of 32 columns need besides the sums: a lane holds one column's scales of each block (and
+// its bias), and each reaches every row of the block by a shuffle.  Loaded before the accumulator is waited for.
+template <int KIND, int BLOCKS>
+struct Scales {
+  using T = Traits<KIND>;
+  float first[T::I8 ? BLOCKS : 1], second[T::I8 ? BLOCKS : 1];
+
+  __device__ __forceinline__ void load(const Args& p, int col, int lane) {
+    if constexpr (T::I8) {
+      const float* other = T::TWO ? p.col_scale1 : p.bias;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; b++) {
+        const int c = col + b * 32 + lane;
+        first[b] = c < p.N ? __ldg(p.col_scale + c) : 0.f;
+        second[b] = other && c < p.N ? __ldg(other + c) : 0.f;
+      }
+    }
+  }
+};
+
+// 32 columns of one accumulator row: sums x, of the up projection y, with the scales k0 and k1 of Scales, to output
+// values v; gated products leave their pre-activations in g and u.
 template <int KIND, int ACT>
-__device__ __forceinline__ void finish32(const Args& p, const uint32_t (&x)[32], const uint32_t (&y)[32], float rs, int col,
-                                         int lane, float (&v)[32], float (&g)[32], float (&u)[32]) {
+__device__ __forceinline__ void finish32(const uint32_t (&x)[32], const uint32_t (&y)[32], float rs, float k0, float k1,
+                                         float (&v)[32], float (&g)[32], float (&u)[32]) {
   using T = Traits<KIND>;
   if constexpr (T::TWO) {
     if constexpr (T::I8) {
-      // a lane holds the scales of one column; each column's reach every row of the block by a shuffle
-      const float cg = col + lane < p.N ? __ldg(p.col_scale + col + lane) : 0.f;
-      const float cu = col + lane < p.N ? __ldg(p.col_scale1 + col + lane) : 0.f;
 #pragma unroll
       for (int j = 0; j < 32; j++) {
-        g[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, cg, j));
-        u[j] = scaled((int32_t)y[j], rs, __shfl_sync(0xffffffffu, cu, j));
+        g[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, k0, j));
+        u[j] = scaled((int32_t)y[j], rs, __shfl_sync(0xffffffffu, k1, j));
       }
     } else {
 #pragma unroll
@@ -672,11 +689,9 @@ __device__ __forceinline__ void finish32(const Args& p, const uint32_t (&x)[32],
 #pragma unroll
     for (int j = 0; j < 32; j++) v[j] = gate<ACT>(g[j]) * u[j];
   } else if constexpr (T::I8) {
-    const float cs = col + lane < p.N ? __ldg(p.col_scale + col + lane) : 0.f;
-    const float add = p.bias && col + lane < p.N ? __ldg(p.bias + col + lane) : 0.f;
 #pragma unroll
     for (int j = 0; j < 32; j++)
-      v[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, cs, j)) + __shfl_sync(0xffffffffu, add, j);
+      v[j] = scaled((int32_t)x[j], rs, __shfl_sync(0xffffffffu, k0, j)) + __shfl_sync(0xffffffffu, k1, j);
   } else {
 #pragma unroll
     for (int j = 0; j < 32; j++) v[j] = __uint_as_float(x[j]);
@@ -879,13 +894,15 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
       float rs = 0.f;
       if constexpr (T::I8)
         if (row < p.M) rs = p.row_scale[row];
+      Scales<KIND, CN / 64> scales;
+      scales.load(p, c0, lane);
       if (!mbar_wait_warp(tfull_bar(acc), acc_phase, abort_flag, WAIT_LIMIT_NS)) {
         if (lane == 0) give_up(74);
         break;
       }
       tc_fence_after();
       const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * PN + part * (CN / 2));
-#pragma unroll 1
+#pragma unroll
       for (int ch = 0; ch < CN / 64; ch++) {
         const int col = c0 + ch * 32;
         uint32_t x[32], y[32], w[BlockStore<O, P_STAGING>::WORDS];
@@ -893,7 +910,7 @@ pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
         tmem_ld_32x32(from + (uint32_t)(ch * 32), x);
         if constexpr (T::TWO) tmem_ld_32x32(from + (uint32_t)(128 + ch * 32), y);
         tmem_ld_wait();
-        finish32<KIND, ACT>(p, x, y, rs, col, lane, v, g, u);
+        finish32<KIND, ACT>(x, y, rs, scales.first[T::I8 ? ch : 0], scales.second[T::I8 ? ch : 0], v, g, u);
         if (KIND == GATED && p.c1) {
           pack<O>(g, w);
           store.put(w, &maps.c1, static_cast<O*>(p.c1), p, row0, col);
@@ -1166,6 +1183,8 @@ tall_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
       float rs = 0.f;
       if constexpr (T::I8)
         if (row < p.M) rs = p.row_scale[row];
+      Scales<KIND, BLOCKS> scales;
+      scales.load(p, c0, lane);
       if (!mbar_wait_warp(tfull_bar(half), acc_phase, abort_flag, WAIT_LIMIT_NS)) {
         if (lane == 0) give_up(85);
         return false;
@@ -1178,7 +1197,7 @@ tall_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
         float v[32];
         tmem_ld_32x32(from + (uint32_t)(b * 32), x);
         tmem_ld_wait();
-        finish32<KIND, 0>(p, x, x, rs, c0 + b * 32, lane, v, v, v);
+        finish32<KIND, 0>(x, x, rs, scales.first[T::I8 ? b : 0], scales.second[T::I8 ? b : 0], v, v, v);
         pack<O>(v, w[b]);
       }
       tc_fence_before();
