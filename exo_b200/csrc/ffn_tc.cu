@@ -247,6 +247,20 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
   return v;
 }
 
+// Sixteen bytes that start `shift` bytes into the aligned vector lo and end in the next one, hi.  Selects, no branches:
+// the shift differs between the rows of a warp.
+__device__ __forceinline__ uint4 join16(const uint4& lo, const uint4& hi, uint32_t shift) {
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  const bool two = shift & 8u, one = shift & 4u;
+#pragma unroll
+  for (int j = 0; j < 6; j++) w[j] = two ? w[j + 2] : w[j];
+#pragma unroll
+  for (int j = 0; j < 5; j++) w[j] = one ? w[j + 1] : w[j];
+  const uint32_t bits = 8 * (shift & 3u);
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
 // One row of an operand as eight lanes share it.
 struct GatherRow {
   const uint8_t* aligned;  // the row's first vector; nullptr: no such row
@@ -266,16 +280,8 @@ struct GatherRow {
   // bytes [at + 16 v, + 16) of the row to their swizzled place in line r of a tile
   __device__ __forceinline__ void place(uint32_t raw, uint32_t tile, int r, int at, int row_bytes, int v) const {
     if (!aligned) return;
-    const uint4 lo = ld_shared16(raw + v * 16), hi = ld_shared16(raw + v * 16 + 16);
-    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    const bool two = shift & 8u, one = shift & 4u;  // differs between the warp's rows: selects, no branches
-#pragma unroll
-    for (int j = 0; j < 6; j++) w[j] = two ? w[j + 2] : w[j];
-#pragma unroll
-    for (int j = 0; j < 5; j++) w[j] = one ? w[j + 1] : w[j];
-    uint32_t y[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) y[j] = __funnelshift_r(w[j], w[j + 1], 8 * (shift & 3u));
+    const uint4 joined = join16(ld_shared16(raw + v * 16), ld_shared16(raw + v * 16 + 16), shift);
+    uint32_t y[4] = {joined.x, joined.y, joined.z, joined.w};
     const int left = row_bytes - at - v * 16;
     if (left < 16) {  // nothing behind the row's end may reach a sum
 #pragma unroll
@@ -1242,7 +1248,8 @@ tall_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Args 
 
 // ------------------------------------------------------------------ operand copies with a pitch that TMA takes
 // TMA reads rows whose pitch and base are multiples of 16 bytes.  Other operands are multiplied from copies with the
-// pitch rounded up; each thread assembles 16 bytes from the aligned words around them.
+// pitch rounded up; each thread assembles 16 bytes from the two aligned vectors around them (bytes behind the row's end
+// are whatever lies there; the tensor map ends before them).
 struct PadJob {
   const uint8_t* src;
   uint8_t* dst;
@@ -1257,18 +1264,16 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ P
   const PadJob& j = jobs.job[blockIdx.y];
   const int64_t per_row = j.dst_pitch / 16, n = j.rows * per_row;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per_row, c = (i - r * per_row) * 16;
+    // (a 64-bit division would take longer than the copy)
+    const int64_t r = n <= UINT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
+    const int64_t c = (i - r * per_row) * 16;
     const uint8_t* s = j.src + r * j.src_pitch + c;
-    const int left = (int)min((int64_t)16, j.src_pitch - c);  // bytes of this row from here on
-    const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(s) & 3u);
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(s - shift);
-    uint32_t x[5];
-#pragma unroll
-    for (int k = 0; k < 5; k++) x[k] = 4 * k < left + (int)shift ? __ldg(w + k) : 0u;  // words that hold a byte of it
-    uint32_t y[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) y[k] = __funnelshift_r(x[k], x[k + 1], 8 * shift);
-    *reinterpret_cast<uint4*>(j.dst + r * j.dst_pitch + c) = make_uint4(y[0], y[1], y[2], y[3]);
+    const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(s) & 15u);
+    const uint4* v = reinterpret_cast<const uint4*>(s - shift);
+    const uint4 lo = __ldg(v);
+    // the second only where it holds a byte of the row
+    const uint4 hi = j.src_pitch - c > 16 - (int)shift ? __ldg(v + 1) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(j.dst + r * j.dst_pitch + c) = join16(lo, hi, shift);
   }
 }
 
@@ -1341,7 +1346,7 @@ cudaError_t make_readable(exo_b200_Context* ctx, StreamMemory& memory, int elem,
     ops[which[c]]->pitch = jobs.job[c].dst_pitch;
     at += jobs.job[c].rows * jobs.job[c].dst_pitch;
   }
-  const unsigned grid = (unsigned)std::min<int64_t>((most + 255) / 256, (int64_t)ctx->sm_count * 8);
+  const unsigned grid = (unsigned)std::min<int64_t>((most + 255) / 256, (int64_t)ctx->sm_count * 16);
   pad_rows_kernel<<<dim3(grid, (unsigned)count), 256, 0, ctx->stream>>>(jobs);
   return cudaGetLastError();
 }
