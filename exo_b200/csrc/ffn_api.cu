@@ -39,6 +39,22 @@ bool bad_act(const char* fn, int_fast32_t act) {
                 "activation must be one of EXO_B200_ACT_SILU, _GELU, _GELU_TANH");
 }
 
+// A thread that is capturing in the strict modes may not allocate, nor ask for much else, until the capture ends; what a
+// first call sets up (the context's status word, its pool, kernel attributes) touches no stream, so it may.
+class RelaxedCapture {
+ public:
+  RelaxedCapture() { exchange(); }
+  ~RelaxedCapture() { exchange(); }
+  RelaxedCapture(const RelaxedCapture&) = delete;
+  RelaxedCapture& operator=(const RelaxedCapture&) = delete;
+
+ private:
+  void exchange() {
+    if (cudaThreadExchangeStreamCaptureMode(&mode_) != cudaSuccess) cudaGetLastError();
+  }
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+};
+
 // The operands of one call: in() and out() take them in any order before anything is enqueued, done() returns the
 // results of host calls.  dev(i) is operand i's device address, nullptr for one that was NULL.
 class Operands {
@@ -132,6 +148,7 @@ class Operands {
   }
 
   const char* fn_;
+  RelaxedCapture relaxed_;  // before the context is looked up
   ContextUse use_;
   Operand op_[kStageSlots];
   bool out_[kStageSlots], on_device_[kStageSlots];

@@ -586,6 +586,97 @@ def test_captured_calls_replay_on_new_inputs(lib, M, F, K):
             assert torch.equal(a, d) and torch.equal(c, d)
 
 
+FIRST_CALL = """
+import sys, torch
+sys.path.insert(0, {root!r})
+import exo_b200
+lib = exo_b200.library()
+M, F, K = 40, 77, 129  # copies of operands, too
+x, w, v = (torch.randn(s, device="cuda").bfloat16() for s in ((M, K), (F, K), (F, K)))
+h, g, u = (torch.zeros(M, F, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+eager = torch.zeros_like(h)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    lib.gated_bf16_exo(None, 0, M, F, K, x, w, v, h, g, u)
+graph.replay()
+torch.cuda.synchronize()
+lib.gated_bf16_exo(None, 0, M, F, K, x, w, v, eager, None, None)
+torch.cuda.synchronize()
+assert torch.equal(h, eager) and float(h.float().abs().sum()) > 0
+print("captured")
+"""
+
+
+@pytest.mark.gpu
+def test_the_first_call_of_a_process_may_be_captured(lib):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.gpu
+def test_threads_share_the_default_context(lib):
+    """Two host threads, each on its own stream with its own operands (copies among them), through the one default
+    context."""
+    import threading
+
+    import torch
+
+    M, F, K = 50, 333, 257
+    x = [dev(bf16_bits(normal(s, (M, K)))) for s in (1, 2)]
+    _, wg, wu = (dev(bf16_bits(t)) for t in gated_inputs(M, F, K))
+    want, got, failed = [], [], []
+    for xi in x:
+        want.append(torch.zeros(M, F, dtype=torch.int16, device="cuda"))
+        got.append([torch.zeros(M, F, dtype=torch.int16, device="cuda") for _ in range(50)])
+        lib.gated_bf16_exo(None, 0, M, F, K, xi, wg, wu, want[-1], None, None)
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for o in got[i]:
+                    lib.gated_bf16_exo(None, 0, M, F, K, x[i], wg, wu, o, None, None)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
+
+
+@pytest.mark.gpu
+def test_infinities_and_nans_stay_in_their_rows(lib):
+    """A token, a channel or a gradient that is not finite spoils its own row or column of the products and no other,
+    at sizes that end inside tiles and vectors."""
+    import torch
+
+    for M, F, K in ((3, 77, 129), (20, 100, 136), (40, 131, 75), (300, 520, 264)):
+        x, wg, wu = (t.copy() for t in gated_inputs(M, F, K))
+        x[1, K - 1] = np.inf
+        wg[F - 1, K - 1] = np.nan
+        h = out((M, F), "bf16")
+        lib.gated_bf16_exo(None, 0, M, F, K, dev(bf16_bits(x)), dev(bf16_bits(wg)), dev(bf16_bits(wu)), h.view, None, None)
+        got = values(h)
+        fine = np.ones((M, F), bool)
+        fine[1] = fine[:, F - 1] = False
+        assert np.isfinite(got[fine]).all() and np.isnan(got[:, F - 1]).all(), (M, F, K)
+        g, u, dh = normal(5, (M, F)), normal(6, (M, F)), normal(7, (M, F), 0.01)
+        dh[M - 1, F - 1] = np.inf
+        x, wg, wu = gated_inputs(M, F, K)
+        res = run_backward(lib, M, F, K, 0, x, wg, wu, g, u, dh)
+        for name, row in (("dx", M - 1), ("dwg", F - 1), ("dwu", F - 1)):
+            ok = np.isfinite(res[name]).all(axis=1)
+            assert not ok[row] and np.delete(ok, row).all(), (name, M, F, K)
+
+
 @pytest.mark.gpu
 def test_host_operands_are_refused_while_capturing(lib):
     import torch
