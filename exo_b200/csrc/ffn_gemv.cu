@@ -379,10 +379,11 @@ cudaError_t launch(exo_b200_Context* ctx, const Problem& p, bool after_own_kerne
   }
   const bool vec = row_bytes % 16 == 0 && aligned16(p.b0) && (KIND == SCALED || aligned16(p.b1));
   const int64_t groups = (p.N + COLS - 1) / COLS;
-  // eight warps an SM keep the memory busy: split rows over the CTA's warps while there are fewer than that
+  // Eight warps an SM, or 24 that have one piece in flight, keep the memory busy: split rows over the CTA's warps while
+  // there are fewer.
   a.k_split = 1;
   const int64_t piece = vec ? 512 : 496, pieces = (row_bytes + piece - 1) / piece;
-  while (a.k_split < WARPS && groups * a.k_split < 8 * ctx->sm_count && pieces >= 2 * a.k_split) a.k_split *= 2;
+  while (a.k_split < WARPS && groups * a.k_split < (vec ? 8 : 24) * ctx->sm_count && pieces >= 2 * a.k_split) a.k_split *= 2;
   const int64_t ctas = (groups * a.k_split + WARPS - 1) / WARPS;
   const size_t smem = (size_t)(p.M * ((row_bytes + 511) / 512 * 512));
   const int per_sm = smem <= 32768 ? 4 : 2;

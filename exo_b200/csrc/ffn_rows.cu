@@ -70,22 +70,47 @@ __global__ void __launch_bounds__(256) quantize_vectors_kernel(int64_t M, int K,
   }
 }
 
-// Any row length and alignment: a CTA or a warp a row, element by element, the second pass out of the caches.
-template <class E, int WARPS>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t M, int64_t K, const E* X, int8_t* Q, float* scale) {
+// Rows of any alignment, element by element but otherwise the same: up to V elements a thread, all on their way at once
+// and kept (a loop over them waits for each: 1283 x 1446 fp32 10.2 us, 5.3 here).
+template <class E, int V, int WARPS>
+__global__ void __launch_bounds__(256) quantize_elements_kernel(int64_t M, int K, const E* X, int8_t* Q, float* scale) {
   grid_dep_launch();
   const int64_t row = (int64_t)blockIdx.x * (8 / WARPS) + threadIdx.x / (32 * WARPS);
-  if (row >= M) return;  // a warp's, or none: a CTA that shares a row has one
+  if (row >= M) return;
   const int t = threadIdx.x % (32 * WARPS);
   const E* x = X + row * K;
   int8_t* q = Q + row * K;
+  float v[V];
   unsigned top = 0;
-#pragma unroll 8
-  for (int64_t k = t; k < K; k += 32 * WARPS) top = max(top, magnitude(float(x[k])));
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int k = t + i * 32 * WARPS;
+    v[i] = k < K ? float(x[k]) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) top = max(top, magnitude(v[i]));
   const Step s = step_of(row_top<WARPS>(top));
   if (t == 0) scale[row] = s.scale;
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int k = t + i * 32 * WARPS;
+    if (k < K) q[k] = (int8_t)quantized(v[i], s);
+  }
+}
+
+// Rows too long for registers: a CTA a row, the second pass out of the caches.
+template <class E>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t K, const E* X, int8_t* Q, float* scale) {
+  grid_dep_launch();
+  const E* x = X + (int64_t)blockIdx.x * K;
+  int8_t* q = Q + (int64_t)blockIdx.x * K;
+  unsigned top = 0;
 #pragma unroll 8
-  for (int64_t k = t; k < K; k += 32 * WARPS) q[k] = (int8_t)quantized(float(x[k]), s);
+  for (int64_t k = threadIdx.x; k < K; k += 256) top = max(top, magnitude(float(x[k])));
+  const Step s = step_of(row_top<8>(top));
+  if (threadIdx.x == 0) scale[blockIdx.x] = s.scale;
+#pragma unroll 8
+  for (int64_t k = threadIdx.x; k < K; k += 256) q[k] = (int8_t)quantized(float(x[k]), s);
 }
 
 template <class E>
@@ -109,10 +134,16 @@ cudaError_t quantize(exo_b200_Context* ctx, int64_t M, int64_t K, const E* X, in
     quantize_vectors_kernel<E, 8, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
   else if (vectors && K <= 4096 * N)
     quantize_vectors_kernel<E, 16, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
-  else if (K <= 1024 && M >= 8 * ctx->sm_count)
-    quantize_rows_kernel<E, 1><<<(m + 7) / 8, 256, 0, st>>>(M, K, X, Q, scale);
+  else if (many && K <= 512)
+    quantize_elements_kernel<E, 16, 1><<<(m + 7) / 8, 256, 0, st>>>(M, (int)K, X, Q, scale);
+  else if (K <= 2048)
+    quantize_elements_kernel<E, 8, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
+  else if (K <= 4096)
+    quantize_elements_kernel<E, 16, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
+  else if (K <= 8192)
+    quantize_elements_kernel<E, 32, 8><<<m, 256, 0, st>>>(M, (int)K, X, Q, scale);
   else
-    quantize_rows_kernel<E, 8><<<m, 256, 0, st>>>(M, K, X, Q, scale);
+    quantize_rows_kernel<E><<<m, 256, 0, st>>>(K, X, Q, scale);
   return cudaGetLastError();
 }
 

@@ -619,23 +619,26 @@ struct BlockStore {
         asm volatile("st.shared.b32 [%0], %1;" ::"r"(area + (uint32_t)(lane * (WORDS + 1) + j) * 4u), "r"(w[j]) : "memory");
       __syncwarp();
       const int rows = min(32, p.M - row0);
-      if (col + lane < p.N) {
-        O* out = C + (int64_t)row0 * p.N + col + lane;
+      if (col + lane >= p.N) return;
+      O* out = C + (int64_t)row0 * p.N + col + lane;
 #pragma unroll 8
-        for (int r = 0; r < rows; r++, out += p.N) {
-          const uint32_t src = area + (uint32_t)(r * (WORDS + 1) * 4 + lane * (int)sizeof(O));
-          if constexpr (sizeof(O) == 2) {
-            uint16_t v;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
-            *reinterpret_cast<uint16_t*>(out) = v;
-          } else {
-            uint32_t v;
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(src) : "memory");
-            *reinterpret_cast<uint32_t*>(out) = v;
-          }
-        }
+      for (int r = 0; r < rows; r++, out += p.N) {
+        const uint32_t v = lds(area + (uint32_t)(r * (WORDS + 1) * 4 + lane * (int)sizeof(O)));
+        if constexpr (sizeof(O) == 2)
+          *reinterpret_cast<uint16_t*>(out) = (uint16_t)v;
+        else
+          *reinterpret_cast<uint32_t*>(out) = v;
       }
     }
+  }
+
+  static __device__ __forceinline__ uint32_t lds(uint32_t a) {  // ordered by the barriers around the block
+    uint32_t v;
+    if constexpr (sizeof(O) == 2)
+      asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v) : "r"(a));
+    else
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
   }
 };
 template <class O, int W>
