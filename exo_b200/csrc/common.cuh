@@ -59,7 +59,8 @@ struct exo_b200_Context {
   exob200::WeightKey wkey;
   // resident CTA pairs of the two cluster kernels on this context's device (0 = not asked yet)
   int max_pairs[4];
-  int max_ffn_pairs, max_ffn_split;  // the same for the feed-forward kernels; largest cluster of their split kernel
+  int max_ffn_pairs;  // the same for the feed-forward pair kernels
+  int ffn_clusters[4];  // clusters of 2, 4, 8, 16 CTAs of the feed-forward split kernel that run at once
   exob200::DeviceStatus* status_dev;   // device word
   exob200::DeviceStatus* status_host;  // pinned mirror
   // host-pointer row pipeline: copy-in / copy-out streams, two chunk buffers each way

@@ -1373,44 +1373,50 @@ bool map_of(CUtensorMap* m, const Matrix& x, int elem, int box_rows) {
     }                                                                                                                 \
   } while (0)
 
-// The largest cluster of the split kernel: MAX_SPLIT where the GPU has room for one (asked once per context, of one
-// instance: all of them take their SM), else eight.
-cudaError_t ask_max_split(exo_b200_Context* ctx, int* most) {
+// How many clusters of 2, 4, 8 and 16 CTAs of the split kernel the GPU holds at once with an SM for each CTA: fewer than
+// its SMs would make, since a cluster stays within one group of them.  Asked once per context, of one instance.
+cudaError_t ask_clusters(exo_b200_Context* ctx) {
   auto* kernel = split_kernel<DGRAD, __nv_bfloat16, 0, false>;
   EXOB200_SMEM_ATTR_ONCE(kernel, S_SMEM_ALONE, ctx->device);
   EXOB200_CLUSTER16_ONCE(kernel, ctx->device);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(MAX_SPLIT);
-  cfg.blockDim = dim3(NUM_THREADS);
-  cfg.dynamicSmemBytes = S_SMEM_ALONE;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = MAX_SPLIT;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-  if (e == cudaSuccess) *most = n >= 4 ? MAX_SPLIT : 8;
-  return e;
-}
-int max_split(exo_b200_Context* ctx) {
-  if (ctx->max_ffn_split == 0 && ask_max_split(ctx, &ctx->max_ffn_split) != cudaSuccess) {
-    cudaGetLastError();
-    ctx->max_ffn_split = 8;
+  for (int i = 0; i < 4; i++) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2u << i;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(2u << i);
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = S_SMEM_ALONE;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&ctx->ffn_clusters[i], kernel, &cfg);
+    if (e != cudaSuccess) return e;
   }
-  return ctx->max_ffn_split;
+  return cudaSuccess;
+}
+// Whether `tiles` clusters of 2^(i + 1) CTAs run at once.
+bool clusters_fit(exo_b200_Context* ctx, int64_t tiles, int i) {
+  if (ctx->ffn_clusters[0] == 0 && ask_clusters(ctx) != cudaSuccess) {
+    cudaGetLastError();
+    for (int k = 0; k < 3; k++) ctx->ffn_clusters[k] = ctx->sm_count / (4 << k);
+    ctx->ffn_clusters[3] = 0;
+  }
+  return tiles <= ctx->ffn_clusters[i];
 }
 
-// How many CTAs of the split kernel share a tile's reduction: as long as every CTA has an SM to itself and two k-blocks.
+// How many CTAs of the split kernel share a tile's reduction: as long as every CTA has an SM to itself, at once, and two
+// k-blocks.
 // (256 x 2048 x 4096 int8, 32 tiles: 14.3, 10.5, 9.5 and 14.8 us with 1, 2, 4 and 8 CTAs a tile; 512 x 2048 x 4096, 64
-// tiles: 14.7, 11.0, 13.0 and 26.7: past one CTA for each SM, and mostly past four of them on one tile, adding up costs
+// tiles: 14.7, 11.0, 13.0 and 26.7; 34 tiles with four, which do not run at once, 13.0, with two 9.2: past one CTA for each SM, and mostly past four of them on one tile, adding up costs
 // more than the shorter loops save.)  A handful of tiles with a long reduction splits further (the gradient of 3 x 177
 // inputs over 2 x 14054 units, two tiles: 33 us of a 60 us backward pass with four, 12.8 with sixteen).
 int split_of(exo_b200_Context* ctx, int64_t tiles, int k_blocks) {
-  int S = 1;
-  while (S < 4 && tiles * S * 2 <= ctx->sm_count && k_blocks / (2 * S) >= 2) S *= 2;
-  while (S >= 4 && S < max_split(ctx) && tiles * S * 4 <= ctx->sm_count && k_blocks / (2 * S) >= 8) S *= 2;
+  int S = 1, i = 0;
+  for (; S < 4 && clusters_fit(ctx, tiles, i) && k_blocks / (2 * S) >= 2; i++) S *= 2;
+  for (; S >= 4 && S < MAX_SPLIT && tiles * S * 4 <= ctx->sm_count && clusters_fit(ctx, tiles, i) &&
+         k_blocks / (2 * S) >= 8; i++)
+    S *= 2;
   return S;
 }
 
@@ -1435,7 +1441,7 @@ int pair_splits(exo_b200_Context* ctx, int64_t rows, int64_t pair_tiles, int64_t
   const double loop = rounds(k_blocks, S);
   const double split = 5.2 + (alone ? 0.30 * loop + (S > 1 ? 0.5 : 0.0) : 0.46 * loop * rounds(split_tiles, 2 * sms));
   const double pair = 6.0 + 0.31 * k_blocks * rounds(pair_tiles, pairs);
-  const double two = pair_tiles * 2 <= pairs && k_blocks >= 2 ? 8.0 + 0.34 * rounds(k_blocks, 2) : 1e30;
+  const double two = clusters_fit(ctx, pair_tiles, 1) && k_blocks >= 2 ? 8.0 + 0.34 * rounds(k_blocks, 2) : 1e30;
   return split <= pair && split <= two ? 0 : pair <= two ? 1 : 2;
 }
 
