@@ -1406,10 +1406,10 @@ bool clusters_fit(exo_b200_Context* ctx, int64_t tiles, int i) {
 }
 
 // How many CTAs of the split kernel share a tile's reduction: as long as every CTA has an SM to itself, at once, and two
-// k-blocks.
-// (256 x 2048 x 4096 int8, 32 tiles: 14.3, 10.5, 9.5 and 14.8 us with 1, 2, 4 and 8 CTAs a tile; 512 x 2048 x 4096, 64
-// tiles: 14.7, 11.0, 13.0 and 26.7; 34 tiles with four, which do not run at once, 13.0, with two 9.2: past one CTA for each SM, and mostly past four of them on one tile, adding up costs
-// more than the shorter loops save.)  A handful of tiles with a long reduction splits further (the gradient of 3 x 177
+// k-blocks.  Past one CTA for each SM, and mostly past four of them on one tile, adding up costs more than the shorter
+// loops save: 256 x 2048 x 4096 int8 (32 tiles) 14.3, 10.5, 9.5 and 14.8 us with 1, 2, 4 and 8 CTAs a tile;
+// 512 x 2048 x 4096 (64 tiles) 14.7, 11.0, 13.0 and 26.7; 16 x 4480 x 4096 (35 tiles, whose clusters of four do not run
+// at once) 9.2 with two, 13.0 with four.  A handful of tiles with a long reduction splits further (the gradient of 3 x 177
 // inputs over 2 x 14054 units, two tiles: 33 us of a 60 us backward pass with four, 12.8 with sixteen).
 int split_of(exo_b200_Context* ctx, int64_t tiles, int k_blocks) {
   int S = 1, i = 0;
@@ -1439,7 +1439,8 @@ int pair_splits(exo_b200_Context* ctx, int64_t rows, int64_t pair_tiles, int64_t
   auto rounds = [](int64_t work, int64_t slots) { return (double)((work + slots - 1) / slots); };
   const bool alone = split_tiles * S <= sms;
   const double loop = rounds(k_blocks, S);
-  const double split = 5.2 + (alone ? 0.30 * loop + (S > 1 ? 0.5 : 0.0) : 0.46 * loop * rounds(split_tiles, 2 * sms));
+  const double turns = rounds(split_tiles, 2 * sms);  // of CTAs that share SMs; each ends in an epilogue of its own
+  const double split = 5.2 + (alone ? 0.30 * loop + (S > 1 ? 0.5 : 0.0) : 0.46 * loop * turns + 5.0 * (turns - 1.0));
   const double pair = 6.0 + 0.31 * k_blocks * rounds(pair_tiles, pairs);
   const double two = clusters_fit(ctx, pair_tiles, 1) && k_blocks >= 2 ? 8.0 + 0.34 * rounds(k_blocks, 2) : 1e30;
   return split <= pair && split <= two ? 0 : pair <= two ? 1 : 2;
