@@ -152,7 +152,8 @@ class CheckedProc(ProcWrapper):
         if _call is not None and current is not None and isinstance(self._dll, ctypes.CDLL):
             address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
             types = tuple(tuple(getattr(torch, n) for n in names) for names in _KINDS.values())
-            _call.setup(torch.Tensor, torch.nn.Parameter, types, current, _last_default_stream, address(self._dll.exo_b200_set_default_stream), address(self._dll.exo_b200_last_error))
+            _call.setup(torch.Tensor, torch.nn.Parameter, types, current, _last_default_stream,
+                        address(self._dll.exo_b200_set_default_stream), address(self._dll.exo_b200_last_error))
             kinds = list(_KINDS)
             self._fast = _call.plan(address(self._fn), self._first - 1,
                                     tuple((kinds.index(kind), d0, d1) for _, kind, _, _, d0, d1 in self._plan))

@@ -24,12 +24,13 @@ PyObject *s_dtype, *s_numel, *s_is_contiguous, *s_data_ptr, *s_get_device, *s_va
 void (*set_default_stream)(void*);
 int (*last_error)();
 
-// setup(Tensor, Parameter, ((dtype, ...), ...) by kind, current raw stream of a device, the cell of the thread's default stream,
-//       address of exo_b200_set_default_stream, address of exo_b200_last_error)
+// setup(Tensor, Parameter, ((dtype, ...), ...) by kind, current raw stream of a device, the cell of the thread's default
+//       stream, address of exo_b200_set_default_stream, address of exo_b200_last_error)
 PyObject* setup(PyObject*, PyObject* args) {
   PyObject *tensor, *parameter, *kinds, *stream, *cell;
   unsigned long long set, last;
-  if (!PyArg_ParseTuple(args, "OOO!OOKK", &tensor, &parameter, &PyTuple_Type, &kinds, &stream, &cell, &set, &last)) return nullptr;
+  if (!PyArg_ParseTuple(args, "OOO!OOKK", &tensor, &parameter, &PyTuple_Type, &kinds, &stream, &cell, &set, &last))
+    return nullptr;
   if (PyTuple_GET_SIZE(kinds) != kKinds) return PyErr_Format(PyExc_ValueError, "expected %d kinds", kKinds);
   for (int k = 0; k < kKinds; k++) {
     PyObject* of = PyTuple_GET_ITEM(kinds, k);
