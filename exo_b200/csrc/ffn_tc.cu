@@ -329,6 +329,7 @@ __device__ __forceinline__ void gather(const Args& p, uint32_t tiles, uint32_t f
   for (int i = 0; i < n_kb; i++) {
     fetch(i + G_DEPTH - 1);  // into the slot that this warp has read in the last round
     cp_async_wait<G_DEPTH - 1>();
+    __syncwarp();  // the wait shows a lane its own copies, and place() reads its neighbour's, too
     // the lanes decide together, so that none is left alone at a barrier
     if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8u * stage, phase, abort_flag, WAIT_LIMIT_NS))) {
       if (lane == 0) report_timeout(p.status, abort_flag, 64);
