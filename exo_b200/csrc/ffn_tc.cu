@@ -532,6 +532,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
                          "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
                          : "memory");
         }
+        __syncwarp();  // lanes of rows past M meet the others before the next load
       }
       tc_fence_before();
     } else if (warp < 6 && lane == 0) {
@@ -619,8 +620,7 @@ struct BlockStore {
       for (int j = 0; j < WORDS; j++)
         asm volatile("st.shared.b32 [%0], %1;" ::"r"(area + (uint32_t)(lane * (WORDS + 1) + j) * 4u), "r"(w[j]) : "memory");
       __syncwarp();
-      const int rows = min(32, p.M - row0);
-      if (col + lane >= p.N) return;
+      const int rows = col + lane < p.N ? min(32, p.M - row0) : 0;
       O* out = C + (int64_t)row0 * p.N + col + lane;
 #pragma unroll 8
       for (int r = 0; r < rows; r++, out += p.N) {
@@ -631,6 +631,7 @@ struct BlockStore {
           *reinterpret_cast<uint32_t*>(out) = v;
       }
     }
+    __syncwarp();  // before the warp's next load of tensor memory
   }
 
   static __device__ __forceinline__ uint32_t lds(uint32_t a) {  // ordered by the barriers around the block
