@@ -59,6 +59,13 @@ constexpr float kRoot2Pi = 0.79788456f;       // sqrt(2 / pi)
 constexpr float kTanhCubic = 0.044715f;
 // beyond this p is 0 or 1 in fp32 for the two GELUs; keeps the cubic and its derivative finite
 constexpr float kGeluClamp = 32.0f;
+// g between -kGeluClamp and kGeluClamp.  A NaN stays one (fminf and fmaxf take the other operand in its place).
+__device__ __forceinline__ float clamped_gate(float g) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(g), "f"(-kGeluClamp));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(c) : "f"(kGeluClamp));
+  return c;
+}
 
 // The normal distribution function by formula 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions
 // (erfc(x) = t (a1 + a2 t + ... + a5 t^4) exp(-x^2), t = 1 / (1 + 0.3275911 x), within 1.5e-7): absolutely as close
@@ -78,7 +85,7 @@ template <int ACT>
 __device__ __forceinline__ float gate_p(float g) {
   if (ACT == EXO_B200_ACT_SILU) return logistic(g);
   if (ACT == EXO_B200_ACT_GELU) return normal_cdf(g);
-  const float c = fminf(fmaxf(g, -kGeluClamp), kGeluClamp);
+  const float c = clamped_gate(g);
   return logistic(2.0f * kRoot2Pi * (c + kTanhCubic * c * c * c));
 }
 template <int ACT>
@@ -90,7 +97,7 @@ template <int ACT>
 __device__ __forceinline__ float gate_slope(float g, float p) {
   if (ACT == EXO_B200_ACT_SILU) return p * (1.0f + g * (1.0f - p));
   if (ACT == EXO_B200_ACT_GELU) return p + g * __expf(-0.5f * g * g) * (0.5f * kRoot2Pi);
-  const float c = fminf(fmaxf(g, -kGeluClamp), kGeluClamp);
+  const float c = clamped_gate(g);
   return p + c * p * (1.0f - p) * (2.0f * kRoot2Pi) * (1.0f + 3.0f * kTanhCubic * c * c);
 }
 
