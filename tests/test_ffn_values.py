@@ -87,3 +87,76 @@ def test_what_is_not_finite_reaches_its_own_gradients(lib, M, F, K, act, value):
         rest = np.ones((M, F), bool)
         rest[m, f] = False
         assert all(np.array_equal(got[k][rest], base[k][rest]) for k in ("dg", "du")), where
+
+
+# ------------------------------------------------------------------ tails
+def tail_of(act):
+    """Negative gates (bf16 values) out to where p(g) leaves fp32's normal range, and p there, from functions that keep
+    their relative accuracy."""
+    end = {"silu": -86.0, "gelu": -12.75, "gelu_tanh": -9.5}[act]
+    g = np.unique(widen(bf16_bits(np.linspace(end, -0.015625, 700).astype(np.float32)))).astype(np.float64)
+    if act == "gelu":
+        p = np.array([0.5 * math.erfc(-v / math.sqrt(2)) for v in g])
+        density = g * np.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    else:
+        c = math.sqrt(2 / math.pi)
+        z = g if act == "silu" else 2 * c * (g + 0.044715 * g ** 3)
+        p = np.exp(z) / (1 + np.exp(z))
+        density = g * p / (1 + np.exp(z)) * (1.0 if act == "silu" else 2 * c * (1 + 3 * 0.044715 * g ** 2))
+    return g, p, density  # act'(g) = p + density
+
+
+# Relative error of p in fp32: the argument of the exponential is at most 88, each of its up to four roundings costs
+# 88 * 2^-24, and so does the product with log2(e) inside; the fast exponential and division 2^-22 each; the fitted
+# coefficients of the normal distribution 2.6e-5.  Together below 6e-5 < 2^-14; the slope adds terms of the same kind.
+TAIL = 2.0 ** -13
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_are_relatively_close_in_their_tails(lib, act, rows):
+    """H = act(g) for gates through a reduction of length one, in the few-row kernel and in the tiles: one bf16 rounding
+    and TAIL, relative to the value itself."""
+    import torch
+
+    g, p, _ = tail_of(act)
+    h = torch.zeros(rows, g.size, dtype=torch.int16, device="cuda")
+    one = np.ones((rows, 1), np.float32)
+    lib.gated_bf16_exo(None, ACTS[act], rows, g.size, 1, dev(one), dev(g[:, None]), dev(np.ones((g.size, 1))), h, None, None)
+    got = widen(h.cpu().numpy().view(np.uint16)).astype(np.float64)
+    want = g * p
+    bad = ~(np.abs(got - want) <= (fo.U16 * (1 + TAIL) + TAIL) * np.abs(want) + fo.TINY16)
+    assert not bad.any(), (g[bad[0]][:4], got[0][bad[0]][:4], want[bad[0]][:4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS)
+def test_slopes_are_relatively_close_in_their_tails(lib, act):
+    """dG = act'(g) and dU = act(g) (dH and U are one): relative to the magnitudes of the two terms of the slope."""
+    g, p, density = tail_of(act)
+    ones = np.ones((1, g.size), np.float32)
+    x, w = np.ones((1, 1), np.float32), np.ones((g.size, 1), np.float32)
+    got = backward(lib, ACTS[act], x, w, w, g[None], ones, ones)
+    for k, want, size in (("dg", p + density, p + np.abs(density)), ("du", g * p, np.abs(g * p))):
+        bad = ~(np.abs(got[k][0] - want) <= fo.U16 * (np.abs(want) + TAIL * size) + TAIL * size + fo.TINY16)
+        assert not bad.any(), (k, g[bad][:4], got[k][0][bad][:4], want[bad][:4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS)
+def test_gates_that_are_not_finite(lib, act):
+    """A NaN token spoils its row of H, an infinite one gives what g p(g) u gives: inf for +inf, NaN or zero for -inf."""
+    import torch
+
+    x = np.array([[np.nan], [np.inf], [-np.inf], [1.0]], np.float32)
+    for rows in (4, 64):
+        a = np.concatenate([x, np.ones((rows - 4, 1), np.float32)])
+        h = torch.zeros(rows, 40, dtype=torch.int16, device="cuda")
+        # the up projection takes a second, finite channel: u = 0 * x would be NaN
+        xs = np.concatenate([a, np.ones((rows, 1), np.float32)], 1)
+        wg, wu = np.tile([[1.0, 0.0]], (40, 1)), np.tile([[1.0, 0.0]], (40, 1))
+        lib.gated_bf16_exo(None, ACTS[act], rows, 40, 2, dev(xs), dev(wg), dev(wu), h, None, None)
+        got = widen(h.cpu().numpy().view(np.uint16))
+        assert np.isnan(got[0]).all() and (got[1] == np.inf).all() and np.isfinite(got[3:]).all()
+        assert (np.isnan(got[2]) | (got[2] == 0)).all()
