@@ -92,6 +92,7 @@ SUPPORT = {
     "exo_b200_set_default_stream": ([vp], None),
     "exo_b200_context_cache_weights": ([vp, ctypes.c_int], None),
     "exo_b200_context_invalidate": ([vp], None),
+    "exo_b200_context_trim": ([vp], None),
     "exo_b200_synchronize": ([vp], ctypes.c_int),
     "exo_b200_selftest_bounded_wait": ([vp, ctypes.c_int], ctypes.c_int),
     "exo_b200_measure_peak": ([ctypes.c_int, ctypes.c_int], ctypes.c_double),

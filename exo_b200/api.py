@@ -238,6 +238,14 @@ class Library:
         if code != OK:
             raise ExoB200Error(code, self.dll.exo_b200_last_error_string().decode())
 
+    def trim(self, ctx: "Context | None" = None) -> None:
+        """Gives the memory that finished calls have left with the context back to the device
+        (exo_b200_context_trim)."""
+        self.dll.exo_b200_context_trim(ctx.handle if ctx else None)
+        code = self.dll.exo_b200_last_error()
+        if code != OK:
+            raise ExoB200Error(code, self.dll.exo_b200_last_error_string().decode())
+
     def version(self) -> str:
         return self.dll.exo_b200_version().decode()
 

@@ -442,6 +442,15 @@ void exo_b200_context_invalidate(exo_b200_Context* ctxt) {
   if (c) c->wkey_valid = false;
 }
 
+void exo_b200_context_trim(exo_b200_Context* ctxt) {
+  clear_error();
+  ContextUse use(resolve_context(ctxt));
+  exo_b200_Context* c = use.get();
+  if (!c) return;
+  if (c->pool && !check_cuda(cudaMemPoolTrimTo(c->pool, 0), "cudaMemPoolTrimTo")) return;
+  check_cuda(cudaDeviceGraphMemTrim(c->device), "cudaDeviceGraphMemTrim");
+}
+
 void exo_b200_set_default_stream(void* stream) { tl_default_stream = static_cast<cudaStream_t>(stream); }
 
 int exo_b200_synchronize(exo_b200_Context* ctxt) {

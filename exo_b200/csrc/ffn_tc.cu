@@ -1303,7 +1303,9 @@ class StreamMemory {
         ctx_->pool = nullptr;
         return e;
       }
-      uint64_t keep = UINT64_MAX;  // freed blocks stay for the next call instead of going back at a synchronisation
+      // Freed blocks stay for the next call, until exo_b200_context_trim: going back at every synchronisation they would
+      // be mapped anew in the call after it.
+      uint64_t keep = UINT64_MAX;
       cudaMemPoolSetAttribute(ctx_->pool, cudaMemPoolAttrReleaseThreshold, &keep);
     }
     cudaError_t e = cudaMallocFromPoolAsync(&p_, bytes, ctx_->pool, ctx_->stream);

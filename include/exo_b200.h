@@ -215,9 +215,12 @@ void ssyrk_exo_3xtf32( void *ctxt, int_fast32_t N, int_fast32_t K, const float* 
  * [N, K] array, tensors are dense and do not alias, sizes are >= 1, pointers are
  * host or device memory and aligned to their element.  bool / enum arguments by value.
  * A call whose operands are all device memory only enqueues and may be captured
- * into a CUDA graph (operand copies that an unaligned pitch needs live in
- * stream-ordered memory that belongs to the call, in a graph to the graph); a call
- * with host operands on a capturing stream is refused (EXO_B200_ERR_UNSUPPORTED).
+ * into a CUDA graph; a call with host operands on a capturing stream is refused
+ * (EXO_B200_ERR_UNSUPPORTED).  A matrix operand of a product whose base or whose
+ * rows' pitch is not a multiple of 16 bytes is copied at every call of more than 32
+ * tokens and at every backward pass: in stream-ordered memory that the call frees and
+ * the context keeps for the next (exo_b200_context_trim gives it back), in a graph in
+ * the graph's own.
  * --------------------------------------------------------------------- */
 
 /* quantize_rows_*_exo: one scale for each row of X.  top = max_k |X[i,k]|:
@@ -291,6 +294,12 @@ void exo_b200_context_set_sgemm_path( exo_b200_Context* ctxt, int path );
  * context of the current device. */
 void exo_b200_context_cache_weights( exo_b200_Context* ctxt, int enable );
 void exo_b200_context_invalidate( exo_b200_Context* ctxt );
+/* The operand copies of the feed-forward calls live in a memory pool of the context, which keeps what it once needed
+ * (the copies of the largest such call, and of each that ran beside it on another stream) for the calls to come.  This
+ * gives that memory back to the device, and what destroyed graphs of such calls have left; copies that enqueued work
+ * still uses stay, so synchronise first.  Later calls allocate again.  ctxt == NULL: the default context of the
+ * current device. */
+void exo_b200_context_trim( exo_b200_Context* ctxt );
 /* Stream used by calls that pass ctxt == NULL (and by the Gemmini-typed calls). */
 void exo_b200_set_default_stream( void* stream );
 /* Wait for the context's stream (NULL: default context) and collect device-side status. */
