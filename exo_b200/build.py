@@ -22,7 +22,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libexo_b200.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
-CALL = os.path.join(HERE, "_call.so")
+# the tag keeps another interpreter from importing it
+CALL = os.path.join(HERE, "_call" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -84,20 +85,44 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+def _remove(path):
+    try:
+        os.remove(path)
+    except FileNotFoundError:
+        pass
+
+
 def build_call(force: bool = False) -> "str | None":
     """The Python binding's fast path (csrc/call.cpp), a plain CPython module.  The package works without it, only
-    slower by a few microseconds a call, so an interpreter without its headers is no error."""
+    slower by a few microseconds a call, so an interpreter without its headers or a machine without a C++ compiler is
+    no error.  What it checks has to be what this source says: modules of an older source, and ones without an
+    interpreter's tag, are removed whether or not a new one can be built."""
     src = os.path.join(CSRC, "call.cpp")
+    for name in os.listdir(os.path.dirname(CALL)):
+        path = os.path.join(os.path.dirname(CALL), name)
+        if name == "_call.so" or (name.startswith("_call.") and name.endswith(".so") and _stale(path, [src])):
+            _remove(path)
+    if not force and os.path.exists(CALL):
+        return CALL
+
+    def without(why):
+        sys.stderr.write(f"exo_b200: the binding's fast path is not built ({why}); calls go through the interpreter\n")
+        _remove(CALL)
+
     headers = sysconfig.get_paths()["include"]
     if not os.path.exists(os.path.join(headers, "Python.h")):
-        return None
-    if force or _stale(CALL, [src]):
-        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I", headers,
-               src, "-o", CALL]
+        return without(f"no Python.h in {headers}")
+    new = f"{CALL}.{os.getpid()}"  # a process may have the old one loaded
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I", headers,
+           src, "-o", new]
+    try:
         r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
-            raise RuntimeError("g++ failed for call.cpp")
+    except OSError as e:
+        return without(str(e))
+    if r.returncode != 0:
+        _remove(new)
+        return without(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+    os.replace(new, CALL)
     return CALL
 
 

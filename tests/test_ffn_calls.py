@@ -1,5 +1,7 @@
 """How the feed-forward entry points are called: memory that calls leave, what the wrapper refuses, the binding's
 build."""
+import os
+
 import numpy as np
 import pytest
 
@@ -69,3 +71,57 @@ def test_trim_gives_the_copies_memory_back(lib):
     torch.cuda.synchronize()
     assert torch.equal(h, again)
     lib.trim()
+
+
+# ------------------------------------------------------------------ build of the binding's fast path
+@pytest.fixture
+def call_at(tmp_path, monkeypatch):
+    """build.build_call into a directory of its own."""
+    import sysconfig
+
+    from exo_b200 import build
+
+    monkeypatch.setattr(build, "CALL", str(tmp_path / os.path.basename(build.CALL)))
+    assert os.path.basename(build.CALL) == "_call" + sysconfig.get_config_var("EXT_SUFFIX")
+    return tmp_path, build
+
+
+def test_the_fast_path_is_built_for_this_interpreter(call_at):
+    import importlib.util
+
+    path, build = call_at
+    (path / "_call.so").write_bytes(b"of some interpreter")
+    (path / "_call.cpython-30-x86_64-linux-gnu.so").write_bytes(b"of another, older than the source")
+    os.utime(path / "_call.cpython-30-x86_64-linux-gnu.so", (1, 1))
+    (path / "_call.cpython-31-x86_64-linux-gnu.so").write_bytes(b"of another")
+    made = build.build_call()
+    assert sorted(os.listdir(path)) == sorted(["_call.cpython-31-x86_64-linux-gnu.so", os.path.basename(made)])
+    spec = importlib.util.spec_from_file_location("_call", made)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    assert callable(module.call)
+    before = os.stat(made).st_mtime_ns
+    assert build.build_call() == made and os.stat(made).st_mtime_ns == before
+
+
+@pytest.mark.parametrize("compiler", ["/nowhere/c++", "false"])
+def test_no_compiler_is_no_error_and_leaves_no_old_module(call_at, monkeypatch, capsys, compiler):
+    path, build = call_at
+    monkeypatch.setenv("CXX", compiler)
+    with open(build.CALL, "wb") as f:
+        f.write(b"of an older source")
+    os.utime(build.CALL, (1, 1))
+    assert build.build_call() is None
+    assert os.listdir(path) == [] and "fast path is not built" in capsys.readouterr().err
+
+
+def test_no_headers_is_no_error_and_leaves_no_old_module(call_at, monkeypatch):
+    import sysconfig
+
+    path, build = call_at
+    with open(build.CALL, "wb") as f:
+        f.write(b"of an older source")
+    os.utime(build.CALL, (1, 1))
+    monkeypatch.setattr(sysconfig, "get_paths", lambda: {"include": str(path / "none")})
+    assert build.build_call() is None
+    assert os.listdir(path) == []
