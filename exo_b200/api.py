@@ -143,16 +143,17 @@ class CheckedProc(ProcWrapper):
         import sys
 
         torch = sys.modules.get("torch")
-        if torch is None:
+        if not hasattr(torch, "Tensor"):  # not there, or still being imported
             return
+        # (torch has uint16 from 2.3 on)
+        known = {kind: tuple(getattr(torch, n) for n in names if hasattr(torch, n)) for kind, names in _KINDS.items()}
         for _, kind, _, types, _, _ in self._plan:
-            types.update(getattr(torch, n) for n in _KINDS[kind])
+            types.update(known[kind])
         self._torch = torch.Tensor
         current = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         if _call is not None and current is not None and isinstance(self._dll, ctypes.CDLL):
             address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
-            types = tuple(tuple(getattr(torch, n) for n in names) for names in _KINDS.values())
-            _call.setup(torch.Tensor, torch.nn.Parameter, types, current, _last_default_stream,
+            _call.setup(torch.Tensor, torch.nn.Parameter, tuple(known.values()), current, _last_default_stream,
                         address(self._dll.exo_b200_set_default_stream), address(self._dll.exo_b200_last_error))
             kinds = list(_KINDS)
             self._fast = _call.plan(address(self._fn), self._first - 1,

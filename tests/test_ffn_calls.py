@@ -125,3 +125,32 @@ def test_no_headers_is_no_error_and_leaves_no_old_module(call_at, monkeypatch):
     monkeypatch.setattr(sysconfig, "get_paths", lambda: {"include": str(path / "none")})
     assert build.build_call() is None
     assert os.listdir(path) == []
+
+
+# ------------------------------------------------------------------ what the wrapper refuses
+def test_a_torch_without_uint16_will_do(lib, monkeypatch):
+    """torch before 2.3 has no uint16, and a module that is still being imported has nothing yet."""
+    import sys
+    import types
+
+    import torch
+
+    import exo_b200
+    from exo_b200 import api
+
+    old = types.ModuleType("torch")
+    for name in ("Tensor", "nn", "bfloat16", "int16", "int8", "float32"):
+        setattr(old, name, getattr(torch, name))
+    old._C = types.SimpleNamespace()
+    for module, torch_known in ((old, True), (types.ModuleType("torch"), False)):
+        monkeypatch.setitem(sys.modules, "torch", module)
+        proc = api.CheckedProc(lib.dll, "gated_bf16_exo")
+        ops = operands("gated_bf16_exo", SIZES["gated_bf16_exo"])
+        with pytest.raises(ValueError, match="has 4 elements"):
+            proc(None, 0, 3, 4, 5, np.ones(4, np.uint16), *ops[1:])
+        with pytest.raises(exo_b200.ExoB200Error):  # arrays pass the wrapper
+            proc(None, 0, 3, 4, 5, None, *ops[1:])
+        if torch_known:
+            tensors = [torch.ones(o.shape, dtype=torch.bfloat16) for o in ops]
+            with pytest.raises(exo_b200.ExoB200Error):
+                proc(None, 0, 3, 4, 5, None, *tensors[1:])
