@@ -123,8 +123,9 @@ _KINDS = {"bf16": ("bfloat16", "int16", "uint16"), "i8": ("int8",), "f32": ("flo
 
 
 class CheckedProc(ProcWrapper):
-    """An entry point whose arrays and tensors are held against its signature (element type, number of elements)
-    before the call: through raw pointers a wrong one would be read or written past its end.  A call of a few
+    """An entry point whose arrays and tensors are held against its signature (element type, number of elements, width
+    of the rows) before the call: through raw pointers a wrong one would be read or written past its end, and a transposed
+    one multiplied wrongly.  One dimension, or any number of them whose last is the row, will do.  A call of a few
     microseconds should not take four times that in its wrapper: torch tensors on a GPU go through the compiled
     ``_call``, everything else through one pass over the arguments here."""
 
@@ -159,12 +160,14 @@ class CheckedProc(ProcWrapper):
             self._fast = _call.plan(address(self._fn), self._first - 1,
                                     tuple((kinds.index(kind), d0, d1) for _, kind, _, _, d0, d1 in self._plan))
 
-    def _refuse(self, at, kind, a, have, count):
+    def _refuse(self, at, kind, a, have, count, width):
         name = f"{self._name}: operand {at - self._first + 1}"
         if have is None:
             raise ValueError(f"{name}: unrecognized type {type(a)}")
         if have != count:
             raise ValueError(f"{name} has {have} elements, not {count}")
+        if width is not None and len(a.shape) > 1 and a.shape[-1] != width:
+            raise ValueError(f"{name} has rows of {a.shape[-1]} elements, not {width}")
         if not (a.flags["C_CONTIGUOUS"] if isinstance(a, np.ndarray) else a.is_contiguous()):
             raise ValueError(f"{name} must be contiguous (dense row-major)")
         raise ValueError(f"{name} holds {a.dtype}, not {kind}")
@@ -192,19 +195,22 @@ class CheckedProc(ProcWrapper):
             a = conv[at]
             if a is None:
                 continue  # a NULL that the entry point does not take is its own refusal
-            count = conv[d0] * conv[d1] if d1 else conv[d0]
+            width = conv[d1] if d1 else None
+            count = conv[d0] * width if d1 else conv[d0]
             if Tensor is not None and isinstance(a, Tensor):
-                if a.dtype not in torch_types or a.numel() != count or not a.is_contiguous():
-                    self._refuse(at, kind, a, a.numel(), count)
+                if (a.dtype not in torch_types or a.numel() != count or not a.is_contiguous()
+                        or d1 and a.dim() > 1 and a.shape[-1] != width):
+                    self._refuse(at, kind, a, a.numel(), count, width)
                 if a.is_cuda and stream is None:
                     stream = _sync_stream_for((a,))
                 conv[at] = a.data_ptr()
             elif isinstance(a, np.ndarray):
-                if a.dtype not in numpy_types or a.size != count or not a.flags["C_CONTIGUOUS"]:
-                    self._refuse(at, kind, a, a.size, count)
+                if (a.dtype not in numpy_types or a.size != count or not a.flags["C_CONTIGUOUS"]
+                        or d1 and a.ndim > 1 and a.shape[-1] != width):
+                    self._refuse(at, kind, a, a.size, count, width)
                 conv[at] = a.ctypes.data
             else:
-                self._refuse(at, kind, a, None, count)
+                self._refuse(at, kind, a, None, count, width)
         ctx = args[0]
         if isinstance(ctx, Context):
             conv[0] = ctx.handle

@@ -20,7 +20,7 @@ struct Plan {
 };
 
 PyObject *tensor_type, *parameter_type, *raw_stream, *stream_cell, *dtypes[kKinds][kMaxTypes];
-PyObject *s_dtype, *s_numel, *s_is_contiguous, *s_data_ptr, *s_get_device, *s_value;
+PyObject *s_dtype, *s_shape, *s_is_contiguous, *s_data_ptr, *s_get_device, *s_value;
 void (*set_default_stream)(void*);
 int (*last_error)();
 
@@ -89,6 +89,31 @@ bool method_int(PyObject* o, PyObject* name, long long* v) {
   return true;
 }
 
+// Whether a tensor has `rows` elements, or `rows` rows of *width of them (in one dimension, or any whose last is the row).
+bool fits(PyObject* o, long long rows, const long long* width) {
+  PyObject* shape = PyObject_GetAttr(o, s_shape);
+  if (!shape || !PyTuple_Check(shape)) {
+    PyErr_Clear();
+    Py_XDECREF(shape);
+    return false;
+  }
+  const Py_ssize_t n = PyTuple_GET_SIZE(shape);
+  __int128 have = 1;  // (a tensor's element count is below 2^63)
+  long long last = 1;
+  for (Py_ssize_t i = 0; i < n; i++) {
+    last = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+    if (last < 0) {
+      PyErr_Clear();
+      Py_DECREF(shape);
+      return false;
+    }
+    have *= last;
+  }
+  Py_DECREF(shape);
+  // sizes that would not fit a product are the Python path's to refuse
+  return have == (__int128)rows * (width ? *width : 1) && (!width || n < 2 || last == *width);
+}
+
 // The thread's default stream as the Python path last set it; sets it where it differs.
 bool use_stream(long long device) {
   PyObject* index = PyLong_FromLongLong(device);
@@ -149,10 +174,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     Py_DECREF(type);  // torch keeps its types
     if (type != dtypes[t.kind][0] && type != dtypes[t.kind][1] && type != dtypes[t.kind][2]) return PyLong_FromLong(-1);
-    // sizes that would not fit a product are the Python path's to refuse
-    const __int128 want = (__int128)v[t.d0] * (t.d1 ? v[t.d1] : 1);
-    long long have, dense;
-    if (!method_int(o, s_numel, &have) || have != want || !method_int(o, s_is_contiguous, &dense) || dense != 1 ||
+    long long dense;
+    if (!fits(o, v[t.d0], t.d1 ? &v[t.d1] : nullptr) || !method_int(o, s_is_contiguous, &dense) || dense != 1 ||
         !method_int(o, s_data_ptr, &v[at]))
       return PyLong_FromLong(-1);
     if (device < 0 && (!method_int(o, s_get_device, &device) || device < 0)) return PyLong_FromLong(-1);
@@ -180,11 +203,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, methods, null
 
 PyMODINIT_FUNC PyInit__call() {
   s_dtype = PyUnicode_InternFromString("dtype");
-  s_numel = PyUnicode_InternFromString("numel");
+  s_shape = PyUnicode_InternFromString("shape");
   s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
   s_data_ptr = PyUnicode_InternFromString("data_ptr");
   s_get_device = PyUnicode_InternFromString("get_device");
   s_value = PyUnicode_InternFromString("value");
-  if (!s_dtype || !s_numel || !s_is_contiguous || !s_data_ptr || !s_get_device || !s_value) return nullptr;
+  if (!s_dtype || !s_shape || !s_is_contiguous || !s_data_ptr || !s_get_device || !s_value) return nullptr;
   return PyModule_Create(&module);
 }

@@ -154,3 +154,72 @@ def test_a_torch_without_uint16_will_do(lib, monkeypatch):
             tensors = [torch.ones(o.shape, dtype=torch.bfloat16) for o in ops]
             with pytest.raises(exo_b200.ExoB200Error):
                 proc(None, 0, 3, 4, 5, None, *tensors[1:])
+
+
+def shapes_of(name, rows, width):
+    """Shapes of rows * width elements, and whether their last dimension is the row."""
+    return [((rows * width,), True), ((rows, width), True), ((1, rows, width), True), ((width, rows), False),
+            ((1, rows * width), False), ((rows * width, 1), False)]
+
+
+def check_shapes(call, name, make):
+    """Every operand of `name` in every shape: the right ones pass the wrapper (and are refused behind it, for an operand
+    that is missing), the others do not."""
+    import exo_b200
+    from exo_b200 import _lib
+
+    sizes = SIZES[name]
+    specs = _lib.SIGNATURES[name][1]
+    ops = [make([sizes[d] for d in dims], kind) for kind, _, dims in specs]
+    required = [i for i, (_, optional, _) in enumerate(specs) if not optional]
+    for i, (kind, _, dims) in enumerate(specs):
+        missing = next(k for k in reversed(required) if k != i)
+        shapes = shapes_of(name, *(sizes[d] for d in dims)) if len(dims) == 2 else [((sizes[dims[0]], 1), True)]
+        for shape, right in shapes:
+            args = [None if k == missing else make(shape, kind) if k == i else o for k, o in enumerate(ops)]
+            if right:
+                with pytest.raises(exo_b200.ExoB200Error) as e:
+                    call(None, *sizes, *args)
+                assert e.value.code == exo_b200.ERR_INVALID_ARGUMENT
+            else:
+                with pytest.raises(ValueError, match=f"operand {i + 1} has rows of {shape[-1]} elements, not"):
+                    call(None, *sizes, *args)
+
+
+TYPES = {"bf16": ("uint16", "bfloat16"), "i8": ("int8", "int8"), "f32": ("float32", "float32")}
+
+
+@pytest.mark.parametrize("name", SIZES)
+def test_wrapper_refuses_transposed_operands(lib, name):
+    """[K, F] where [F, K] is meant has the right count and the wrong rows."""
+    import torch
+
+    check_shapes(getattr(lib, name), name, lambda shape, kind: np.ones(shape, TYPES[kind][0]))
+    check_shapes(getattr(lib, name), name, lambda shape, kind: torch.ones(shape, dtype=getattr(torch, TYPES[kind][1])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", SIZES)
+def test_wrapper_refuses_transposed_device_operands(lib, name):
+    import torch
+
+    check_shapes(getattr(lib, name), name,
+                 lambda shape, kind: torch.ones(shape, dtype=getattr(torch, TYPES[kind][1]), device="cuda"))
+    assert getattr(lib, name)._fast is not None
+
+
+@pytest.mark.gpu
+def test_the_fast_path_takes_every_right_shape(lib):
+    import torch
+
+    from exo_b200 import api
+
+    x, s = torch.randn(6, 8, device="cuda"), torch.zeros(6, device="cuda")
+    q = torch.zeros(6, 8, dtype=torch.int8, device="cuda")
+    lib.quantize_rows_f32_exo(None, 6, 8, x, q, s)
+    for shape in ((48,), (6, 8), (2, 3, 8), (1, 6, 8)):
+        again, t = torch.zeros_like(q).view(shape), torch.zeros(3, 2, device="cuda")
+        assert api._call.call(lib.quantize_rows_f32_exo._fast, (None, 6, 8, x.view(shape), again, t)) == 0
+        assert torch.equal(again.view(6, 8), q) and torch.equal(t.view(6), s)
+    for shape in ((8, 6), (48, 1), (1, 48), (2, 4, 6)):
+        assert api._call.call(lib.quantize_rows_f32_exo._fast, (None, 6, 8, x.view(shape), q, s)) == -1
