@@ -204,6 +204,8 @@ class CheckedProc(ProcWrapper):
                 if a.is_cuda and stream is None:
                     stream = _sync_stream_for((a,))
                 conv[at] = a.data_ptr()
+                if not conv[at] and count:  # a meta tensor, which would pass for an operand that is left out
+                    raise ValueError(f"{self._name}: operand {at - self._first + 1} has no memory ({a.device})")
             elif isinstance(a, np.ndarray):
                 if (a.dtype not in numpy_types or a.size != count or not a.flags["C_CONTIGUOUS"]
                         or d1 and a.ndim > 1 and a.shape[-1] != width):

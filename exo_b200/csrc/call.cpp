@@ -176,7 +176,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (type != dtypes[t.kind][0] && type != dtypes[t.kind][1] && type != dtypes[t.kind][2]) return PyLong_FromLong(-1);
     long long dense;
     if (!fits(o, v[t.d0], t.d1 ? &v[t.d1] : nullptr) || !method_int(o, s_is_contiguous, &dense) || dense != 1 ||
-        !method_int(o, s_data_ptr, &v[at]))
+        !method_int(o, s_data_ptr, &v[at]) || !v[at])  // (no memory: not the same as no operand)
       return PyLong_FromLong(-1);
     if (device < 0 && (!method_int(o, s_get_device, &device) || device < 0)) return PyLong_FromLong(-1);
   }

@@ -223,3 +223,30 @@ def test_the_fast_path_takes_every_right_shape(lib):
         assert torch.equal(again.view(6, 8), q) and torch.equal(t.view(6), s)
     for shape in ((8, 6), (48, 1), (1, 48), (2, 4, 6)):
         assert api._call.call(lib.quantize_rows_f32_exo._fast, (None, 6, 8, x.view(shape), q, s)) == -1
+
+
+@pytest.mark.parametrize("name", SIZES)
+def test_wrapper_refuses_tensors_without_memory(lib, name):
+    """A meta tensor has an address of zero, which an optional operand would take for None."""
+    import torch
+
+    ops = operands(name, SIZES[name])
+    for i, o in enumerate(ops):
+        meta = torch.ones(o.shape, dtype={"uint16": torch.bfloat16}.get(str(o.dtype), getattr(torch, str(o.dtype))),
+                          device="meta")
+        with pytest.raises(ValueError, match=f"operand {i + 1} has no memory"):
+            getattr(lib, name)(None, *SIZES[name], *ops[:i], meta, *ops[i + 1:])
+
+
+@pytest.mark.gpu
+def test_wrapper_refuses_a_bias_without_memory(lib):
+    """The same beside operands on the GPU, where the compiled path makes the calls."""
+    import torch
+
+    a, s = torch.ones(3, 5, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda")
+    c = torch.zeros(3, 3, device="cuda")
+    lib.gemm_i8_scaled_f32_exo(None, 3, 3, 5, a, a, s, s, None, c)
+    c.zero_()
+    with pytest.raises(ValueError, match="operand 5 has no memory"):
+        lib.gemm_i8_scaled_f32_exo(None, 3, 3, 5, a, a, s, s, torch.ones(3, device="meta"), c)
+    assert not c.any()
