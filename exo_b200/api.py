@@ -190,6 +190,8 @@ class CheckedProc(ProcWrapper):
         for i in range(1, self._first):
             if type(conv[i]) is not int:
                 conv[i] = operator.index(conv[i])
+            if not -1 << 63 <= conv[i] < 1 << 63:  # ctypes would pass its low 64 bits
+                raise ValueError(f"{self._name}: argument {i} is out of range")
         stream = None
         for at, kind, numpy_types, torch_types, d0, d1 in self._plan:
             a = conv[at]

@@ -250,3 +250,21 @@ def test_wrapper_refuses_a_bias_without_memory(lib):
     with pytest.raises(ValueError, match="operand 5 has no memory"):
         lib.gemm_i8_scaled_f32_exo(None, 3, 3, 5, a, a, s, s, torch.ones(3, device="meta"), c)
     assert not c.any()
+
+
+@pytest.mark.parametrize("name", SIZES)
+def test_wrapper_refuses_numbers_beyond_64_bits(lib, name):
+    """2^64 is 0 in 64 bits: an activation of that number was SiLU."""
+    import torch
+
+    ops = operands(name, SIZES[name])
+    for i, size in enumerate(SIZES[name]):
+        for wrong in (size + 2 ** 64, size - 2 ** 64, 2 ** 63, -2 ** 63 - 1):
+            with pytest.raises(ValueError, match="out of range"):
+                getattr(lib, name)(None, *SIZES[name][:i], wrong, *SIZES[name][i + 1:], *ops)
+    if torch.cuda.is_available():
+        return
+    import exo_b200
+
+    with pytest.raises(exo_b200.ExoB200Error):  # any integer type will do otherwise
+        getattr(lib, name)(None, *(np.int32(s) for s in SIZES[name]), *ops)
