@@ -57,31 +57,35 @@ for _n in _CONV_INSTANCES:
     PROTOTYPES[f"conv_{_n}"] = [vp, vp, vp, vp, vp, cbool, vp]
 
 # Element type and shape (as names of the sizes) of every tensor of the feed-forward entry points, in order; "?"
-# marks one that may be None.  The wrapper holds arrays and tensors against these before the call.
-_LINEAR = "M N K", "{t} M K, i8 N K, f32 N, f32? N, i8 M K, f32 M, {t} M N"
-_SCALED = "M N K", "i8 M K, i8 N K, f32 M, f32 N, f32? N, {t} M N"
+# marks one that may be None, "=" one that is written.  The wrapper holds arrays and tensors against these before the
+# call.
+_LINEAR = "M N K", "{t} M K, i8 N K, f32 N, f32? N, =i8 M K, =f32 M, ={t} M N"
+_SCALED = "M N K", "i8 M K, i8 N K, f32 M, f32 N, f32? N, ={t} M N"
 
 
 def _signature(sizes, tensors, t=""):
-    specs = []
-    for spec in tensors.format(t=t).split(","):
+    """(number of sizes, (element type, may be None, its sizes) of each tensor, positions of the ones that are written)"""
+    specs, written = [], set()
+    for at, spec in enumerate(tensors.format(t=t).split(",")):
         kind, *dims = spec.split()
-        specs.append((kind.rstrip("?"), kind.endswith("?"), tuple(sizes.split().index(d) for d in dims)))
-    return len(sizes.split()), tuple(specs)
+        specs.append((kind.strip("=?"), kind.endswith("?"), tuple(sizes.split().index(d) for d in dims)))
+        if kind.startswith("="):
+            written.add(at)
+    return len(sizes.split()), tuple(specs), frozenset(written)
 
 
 SIGNATURES = {
-    "quantize_rows_bf16_exo": _signature("M K", "bf16 M K, i8 M K, f32 M"),
-    "quantize_rows_f32_exo": _signature("M K", "f32 M K, i8 M K, f32 M"),
+    "quantize_rows_bf16_exo": _signature("M K", "bf16 M K, =i8 M K, =f32 M"),
+    "quantize_rows_f32_exo": _signature("M K", "f32 M K, =i8 M K, =f32 M"),
     "gemm_i8_scaled_bf16_exo": _signature(*_SCALED, "bf16"),
     "gemm_i8_scaled_f32_exo": _signature(*_SCALED, "f32"),
     "linear_i8_bf16_exo": _signature(*_LINEAR, "bf16"),
     "linear_i8_f32_exo": _signature(*_LINEAR, "f32"),
-    "gated_bf16_exo": _signature("act M F K", "bf16 M K, bf16 F K, bf16 F K, bf16 M F, bf16? M F, bf16? M F"),
+    "gated_bf16_exo": _signature("act M F K", "bf16 M K, bf16 F K, bf16 F K, =bf16 M F, =bf16? M F, =bf16? M F"),
     "gated_bf16_backward_exo": _signature(
-        "act M F K", "bf16 M K, bf16 F K, bf16 F K, bf16 M F, bf16 M F, bf16 M F, bf16 M F, bf16 M F, "
-                     "bf16? M K, bf16? F K, bf16? F K"),
-    "gated_i8_bf16_exo": _signature("act M F K", "i8 M K, i8 F K, i8 F K, f32 M, f32 F, f32 F, bf16 M F"),
+        "act M F K", "bf16 M K, bf16 F K, bf16 F K, bf16 M F, bf16 M F, bf16 M F, =bf16 M F, =bf16 M F, "
+                     "=bf16? M K, =bf16? F K, =bf16? F K"),
+    "gated_i8_bf16_exo": _signature("act M F K", "i8 M K, i8 F K, i8 F K, f32 M, f32 F, f32 F, =bf16 M F"),
 }
 
 SUPPORT = {

@@ -131,8 +131,9 @@ class CheckedProc(ProcWrapper):
 
     def __init__(self, dll, name):
         super().__init__(dll, name)
-        sizes, tensors = _lib.SIGNATURES[name]
+        sizes, tensors, written = _lib.SIGNATURES[name]
         self._first = 1 + sizes
+        self._written = frozenset(1 + sizes + i for i in written)
         numpy_types = {k: frozenset(np.dtype(n) for n in names if n != "bfloat16") for k, names in _KINDS.items()}
         # per tensor: position, kind, numpy types, torch types (filled in when torch is there), its one or two sizes
         self._plan = [(1 + sizes + i, kind, numpy_types[kind], set(), 1 + dims[0], 1 + dims[1] if len(dims) > 1 else 0)
@@ -212,6 +213,8 @@ class CheckedProc(ProcWrapper):
                 if (a.dtype not in numpy_types or a.size != count or not a.flags["C_CONTIGUOUS"]
                         or d1 and a.ndim > 1 and a.shape[-1] != width):
                     self._refuse(at, kind, a, a.size, count, width)
+                if at in self._written and not a.flags.writeable:
+                    raise ValueError(f"{self._name}: operand {at - self._first + 1} is written, and the array is read-only")
                 conv[at] = a.ctypes.data
             else:
                 self._refuse(at, kind, a, None, count, width)

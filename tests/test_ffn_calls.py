@@ -268,3 +268,28 @@ def test_wrapper_refuses_numbers_beyond_64_bits(lib, name):
 
     with pytest.raises(exo_b200.ExoB200Error):  # any integer type will do otherwise
         getattr(lib, name)(None, *(np.int32(s) for s in SIZES[name]), *ops)
+
+
+@pytest.mark.parametrize("name", SIZES)
+def test_wrapper_refuses_to_write_read_only_arrays(lib, name):
+    """Results do not go into arrays that numpy itself would not write (a file mapped for reading, a view of bytes);
+    inputs may be such."""
+    import torch
+
+    import exo_b200
+
+    first_output = {"quantize_rows": 1, "gemm_i8_scaled": 5, "linear_i8": 4, "gated_bf16_exo": 3,
+                    "gated_bf16_backward_exo": 6, "gated_i8_bf16_exo": 6}
+    first = next(v for k, v in first_output.items() if name.startswith(k))
+    ops = operands(name, SIZES[name])
+    for i, o in enumerate(ops):
+        fixed = np.frombuffer(o.tobytes(), o.dtype).reshape(o.shape)
+        assert not fixed.flags.writeable
+        args = (None, *SIZES[name], *ops[:i], fixed, *ops[i + 1:])
+        if i >= first:
+            with pytest.raises(ValueError, match=f"operand {i + 1} is written"):
+                getattr(lib, name)(*args)
+        elif not torch.cuda.is_available():
+            with pytest.raises(exo_b200.ExoB200Error):  # past the wrapper: there is no device
+                getattr(lib, name)(*args)
+        assert (fixed == 1).all()
