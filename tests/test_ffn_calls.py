@@ -73,6 +73,90 @@ def test_trim_gives_the_copies_memory_back(lib):
     lib.trim()
 
 
+@pytest.mark.gpu
+def test_graphs_with_copies_run_beside_one_another(lib):
+    """Two graphs whose calls copy operands, replayed on two streams at once, trimmed in between, while eager calls of
+    another size go through a third stream: each has memory of its own."""
+    import torch
+
+    M, F, K = 200, 1333, 517
+    wg, wu = (torch.randn(F, K, device="cuda").bfloat16() * 0.05 for _ in range(2))
+    x = [torch.randn(M, K, device="cuda").bfloat16() for _ in range(2)]
+    want, got = ([torch.zeros(M, F, dtype=torch.bfloat16, device="cuda") for _ in range(2)] for _ in range(2))
+    big = [torch.randn(s, device="cuda").bfloat16() for s in ((300, 519), (2000, 519), (2000, 519))]
+    other, other_want = (torch.zeros(300, 2000, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    for xi, w in zip(x, want):
+        lib.gated_bf16_exo(None, 1, M, F, K, xi, wg, wu, w, None, None)
+    lib.gated_bf16_exo(None, 1, 300, 2000, 519, *big, other_want, None, None)
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(3)]
+    for xi, g in zip(x, got):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            lib.gated_bf16_exo(None, 1, M, F, K, xi, wg, wu, g, None, None)
+        graphs.append(graph)
+    for round in range(10):
+        for g in (*got, other):
+            g.zero_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            with torch.cuda.stream(streams[2]):
+                lib.gated_bf16_exo(None, 1, 300, 2000, 519, *big, other, None, None)
+        if round % 3 == 1:
+            lib.trim()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(other, other_want)
+        if round % 3 == 2:
+            lib.trim()
+
+
+@pytest.mark.gpu
+def test_a_thread_may_capture_while_another_calls(lib):
+    """One thread captures calls with copies while another one's calls grow the context's pool."""
+    import threading
+
+    import torch
+
+    M, F, K = 64, 333, 257
+    x, wg, wu = (torch.randn(s, device="cuda").bfloat16() for s in ((M, K), (F, K), (F, K)))
+    h, want = (torch.zeros(M, F, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    lib.gated_bf16_exo(None, 0, M, F, K, x, wg, wu, want, None, None)
+    big = [torch.randn(s, device="cuda").bfloat16() for s in ((64, 1001), (9001, 1001), (9001, 1001))]
+    wide, wide_want = (torch.zeros(64, 9001, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    lib.gated_bf16_exo(None, 0, 64, 9001, 1001, *big, wide_want, None, None)
+    torch.cuda.synchronize()
+    lib.trim()
+    captured, called, failed = threading.Event(), threading.Event(), []
+
+    def work():
+        try:
+            captured.wait(60)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(3):
+                    lib.gated_bf16_exo(None, 0, 64, 9001, 1001, *big, wide, None, None)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+        finally:
+            called.set()
+
+    thread = threading.Thread(target=work)
+    thread.start()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        lib.gated_bf16_exo(None, 0, M, F, K, x, wg, wu, h, None, None)
+        captured.set()
+        assert called.wait(60)
+        lib.gated_bf16_exo(None, 0, M, F, K, x, wg, wu, h, None, None)
+    thread.join()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    assert torch.equal(h, want) and torch.equal(wide, wide_want)
+
+
 # ------------------------------------------------------------------ build of the binding's fast path
 @pytest.fixture
 def call_at(tmp_path, monkeypatch):
