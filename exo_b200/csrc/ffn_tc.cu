@@ -620,11 +620,13 @@ struct BlockStore {
       for (int j = 0; j < WORDS; j++)
         asm volatile("st.shared.b32 [%0], %1;" ::"r"(area + (uint32_t)(lane * (WORDS + 1) + j) * 4u), "r"(w[j]) : "memory");
       __syncwarp();
-      const int rows = col + lane < p.N ? min(32, p.M - row0) : 0;
+      const int rows = min(32, p.M - row0);  // the same for all lanes: those past N go along and store nothing
+      const bool in = col + lane < p.N;
       O* out = C + (int64_t)row0 * p.N + col + lane;
 #pragma unroll 8
       for (int r = 0; r < rows; r++, out += p.N) {
         const uint32_t v = lds(area + (uint32_t)(r * (WORDS + 1) * 4 + lane * (int)sizeof(O)));
+        if (!in) continue;
         if constexpr (sizeof(O) == 2)
           *reinterpret_cast<uint16_t*>(out) = (uint16_t)v;
         else
