@@ -101,18 +101,27 @@ class ProcWrapper:
         if len(args) != len(self._argtypes):
             raise TypeError(f"{self._name} takes {len(self._argtypes)} arguments ({len(args)} given)")
         stream = _sync_stream_for(args)
-        ctx = args[0] if isinstance(args[0], Context) else None
-        if ctx is not None:
-            if stream is not None:
-                self._dll.exo_b200_context_set_stream(ctx.handle, stream)
-        elif getattr(_last_default_stream, "value", -1) != stream:
-            # the library keeps the default stream per host thread; tell it only when it changes
-            self._dll.exo_b200_set_default_stream(stream)
-            _last_default_stream.value = stream
         keepalive = []  # per call, so concurrent callers cannot free each other's scalars
         conv = [_convert(a, t, keepalive) for a, t in zip(args, self._argtypes)]
-        self._fn(*conv)
+        self._enqueue(args[0] if isinstance(args[0], Context) else None, stream, conv)
         del keepalive
+
+    def _enqueue(self, ctx, stream, conv):
+        """The call itself, on `stream` (None: no operand is on a GPU).  A context that has been closed is none."""
+        if ctx is not None and ctx.handle:
+            with ctx.lock:  # neither another thread's stream nor its close() may come between
+                conv[0] = ctx.handle
+                if stream is not None and conv[0]:
+                    self._dll.exo_b200_context_set_stream(conv[0], stream)
+                self._fn(*conv)
+        else:
+            if ctx is not None:
+                conv[0] = None
+            if getattr(_last_default_stream, "value", -1) != stream:
+                # the library keeps the default stream per host thread; tell it only when it changes
+                self._dll.exo_b200_set_default_stream(stream)
+                _last_default_stream.value = stream
+            self._fn(*conv)
         code = self._dll.exo_b200_last_error()
         if code != OK:
             raise ExoB200Error(code, self._dll.exo_b200_last_error_string().decode())
@@ -219,19 +228,9 @@ class CheckedProc(ProcWrapper):
             else:
                 self._refuse(at, kind, a, None, count, width)
         ctx = args[0]
-        if isinstance(ctx, Context):
-            conv[0] = ctx.handle
-            if stream is not None:
-                self._dll.exo_b200_context_set_stream(ctx.handle, stream)
-        elif ctx is not None:
+        if ctx is not None and not isinstance(ctx, Context):
             raise ValueError(f"unrecognized type {type(ctx)}")
-        elif getattr(_last_default_stream, "value", -1) != stream:
-            self._dll.exo_b200_set_default_stream(stream)
-            _last_default_stream.value = stream
-        self._fn(*conv)
-        code = self._dll.exo_b200_last_error()
-        if code != OK:
-            raise ExoB200Error(code, self._dll.exo_b200_last_error_string().decode())
+        self._enqueue(ctx, stream, conv)
 
 
 class Library:
@@ -267,7 +266,10 @@ class Library:
 class Context:
     """An explicit context: device, stream and SGEMM arithmetic path."""
 
+    handle = None
+
     def __init__(self, device: int = -1, stream: int | None = None, sgemm_path: int = SGEMM_FFMA):
+        self.lock = threading.Lock()  # held while a thread sets the stream and makes its call
         self._dll = _lib.load()
         self.handle = self._dll.exo_b200_context_create(device, stream)
         if not self.handle:
@@ -277,8 +279,10 @@ class Context:
 
     def close(self):
         if self.handle:
-            self._dll.exo_b200_context_destroy(self.handle)
-            self.handle = None
+            with self.lock:
+                handle, self.handle = self.handle, None
+                if handle:
+                    self._dll.exo_b200_context_destroy(handle)
 
     def __del__(self):
         try:

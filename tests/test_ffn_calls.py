@@ -377,3 +377,132 @@ def test_wrapper_refuses_to_write_read_only_arrays(lib, name):
             with pytest.raises(exo_b200.ExoB200Error):  # past the wrapper: there is no device
                 getattr(lib, name)(*args)
         assert (fixed == 1).all()
+
+
+# ------------------------------------------------------------------ contexts and threads
+class RecordingLibrary:
+    """Stands for the library: remembers on which stream each call would have run."""
+
+    def __init__(self):
+        self.context_stream, self.default_stream, self.calls = None, None, []
+
+    def exo_b200_context_set_stream(self, handle, stream):
+        import time
+
+        self.context_stream = stream
+        time.sleep(0.002)  # another thread's chance
+
+    def exo_b200_set_default_stream(self, stream):
+        self.default_stream = stream
+
+    def exo_b200_last_error(self):
+        return 0
+
+    def exo_b200_context_destroy(self, handle):
+        pass
+
+    def __getattr__(self, name):
+        def call(ctx, *args):
+            self.calls.append((args[0], self.context_stream if ctx else self.default_stream))
+
+        return call
+
+
+def recording(monkeypatch, wrapper, name):
+    """(library, context, f(context, stream, mark)) with a wrapper whose operands claim to be on a GPU."""
+    import ctypes
+    import threading
+
+    import torch
+
+    import exo_b200
+    from exo_b200 import api
+
+    class OnDevice(torch.Tensor):
+        is_cuda = property(lambda self: True)
+        __module__ = "torch"  # what the wrapper without checks goes by
+
+    current, dll = threading.local(), RecordingLibrary()
+    monkeypatch.setattr(api, "_sync_stream_for", lambda args: current.stream)
+    monkeypatch.setattr(api, "_last_default_stream", threading.local())
+    context = exo_b200.Context.__new__(exo_b200.Context)
+    context.lock, context.handle, context._dll = threading.Lock(), 7, dll
+    proc = wrapper(dll, name)
+
+    def make(ctx, stream, mark):
+        current.stream = stream
+        shapes = {"quantize_rows_f32_exo": ((mark, 2), (mark, 2), (mark,)), "gemm_bf16_exo": ((mark, 2), (2, 2), (mark, 2))}
+        types = {"quantize_rows_f32_exo": (torch.float32, torch.int8, torch.float32), "gemm_bf16_exo": (torch.bfloat16,) * 3}
+        ops = [torch.zeros(s, dtype=t).as_subclass(OnDevice) for s, t in zip(shapes[name], types[name])]
+        proc(ctx, *((mark, 2) if len(proc._argtypes) == 6 else (mark, 2, 2)), *ops)
+
+    return dll, context, make
+
+
+@pytest.mark.parametrize("wrapper,name", [("CheckedProc", "quantize_rows_f32_exo"), ("ProcWrapper", "gemm_bf16_exo")])
+def test_threads_that_share_a_context_keep_their_streams(monkeypatch, wrapper, name):
+    """Host threads may share a context: setting its stream and the call are one step."""
+    import threading
+
+    from exo_b200 import api
+
+    dll, context, make = recording(monkeypatch, getattr(api, wrapper), name)
+    threads = [threading.Thread(target=lambda i=i: [make(context, 1000 + i, i) for _ in range(20)]) for i in (1, 2, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(dll.calls) == 60 and all(stream == 1000 + mark for mark, stream in dll.calls)
+
+
+@pytest.mark.parametrize("wrapper,name", [("CheckedProc", "quantize_rows_f32_exo"), ("ProcWrapper", "gemm_bf16_exo")])
+def test_a_closed_context_is_the_default_one_on_the_callers_stream(monkeypatch, wrapper, name):
+    from exo_b200 import api
+
+    dll, context, make = recording(monkeypatch, getattr(api, wrapper), name)
+    make(None, 11, 1)
+    make(context, 22, 2)
+    context.close()
+    make(context, 33, 3)
+    assert dll.calls == [(1, 11), (2, 22), (3, 33)]
+
+
+@pytest.mark.gpu
+def test_threads_share_a_context(lib):
+    """Two host threads, each on its own stream with its own operands, through one explicit context."""
+    import threading
+
+    import torch
+
+    import exo_b200
+
+    M, F, K = 50, 333, 257
+    wg, wu = (torch.randn(F, K, device="cuda").bfloat16() for _ in range(2))
+    want, got, failed = [], [], []
+    ctx = exo_b200.Context()
+    sources = [torch.randn(M, K, device="cuda").bfloat16() for _ in range(2)]
+    for x in sources:
+        want.append(torch.zeros(M, F, dtype=torch.bfloat16, device="cuda"))
+        got.append([torch.zeros(M, F, dtype=torch.bfloat16, device="cuda") for _ in range(50)])
+        lib.gated_bf16_exo(None, 0, M, F, K, x, wg, wu, want[-1], None, None)
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for o in got[i]:
+                    x = sources[i] * 1  # written on this thread's stream just before the call reads it
+                    lib.gated_bf16_exo(ctx, 0, M, F, K, x, wg, wu, o, None, None)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
