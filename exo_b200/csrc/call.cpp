@@ -1,7 +1,7 @@
 // The calls of the checked entry points (exo_b200/api.py, CheckedProc) for the ordinary case: no context, and torch
-// tensors of the right types and sizes, the first of them on a GPU.  The interpreter and ctypes take 5 us for such a
-// call, as long as the launch behind it; this takes 1 us (linear_i8_bf16_exo on 11 arguments,
-// launch included: 6.5 us, 9.6 through the interpreter).  Whatever is not the ordinary case is left to the Python
+// tensors of the right types and sizes, the first of them on a GPU.  The interpreter and ctypes take 5.5 us for
+// such a call, longer than the launch behind it; this takes 2 us (linear_i8_bf16_exo on 11 arguments, launch included:
+// 6.1 us, 9.7 through the interpreter).  Whatever is not the ordinary case is left to the Python
 // path, which also finds the words for what is wrong.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>

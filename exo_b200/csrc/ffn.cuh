@@ -34,7 +34,10 @@ cudaError_t launch_quantize_rows(exo_b200_Context* ctx, int64_t M, int64_t K, co
 // way (or waits for one that was), so this one may be scheduled before it ends.
 cudaError_t launch_product(exo_b200_Context* ctx, Kind kind, bool out_f32, const Problem& p, bool after_own_kernel);
 // dX = dG Wg + dU Wu [M,K] and dWg = dG^T X, dWu = dU^T X [F,K], each only where it is wanted (dWg and dWu together);
-// after launch_gate_backward on the same stream.
+// after launch_gate_backward on the same stream.  dG and dU enter as rounded to bf16, the type that the tensor core
+// multiplies: the gradients are 2.3e-3 of their norm from exact, 1.7e-3 of it their own rounding.  Entering unrounded, as
+// sums of two bf16 numbers, they would come to 1.7e-3 for twice the products (a training step's backward pass of 8192 x
+// 8192 x 4096 is 1.6 ms of products in 1.7).
 cudaError_t launch_gradients(exo_b200_Context* ctx, int64_t M, int64_t F, int64_t K, const void* X, const void* Wg,
                              const void* Wu, const void* dG, const void* dU, void* dX, void* dWg, void* dWu);
 // The products of a few rows (ffn_gemv.cu): whether they are taken for a problem, and their launch.

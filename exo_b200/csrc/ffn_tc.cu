@@ -1306,7 +1306,7 @@ class StreamMemory {
         return e;
       }
       // Freed blocks stay for the next call, until exo_b200_context_trim: going back at every synchronisation they would
-      // be mapped anew in the call after it.
+      // be mapped anew in the call after it (64 x 16384 x 4095 gated, 268 MB of copies: 155 us, 2 to 4 ms when mapped).
       uint64_t keep = UINT64_MAX;
       cudaMemPoolSetAttribute(ctx_->pool, cudaMemPoolAttrReleaseThreshold, &keep);
     }

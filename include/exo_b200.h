@@ -214,6 +214,9 @@ void ssyrk_exo_3xtf32( void *ctxt, int_fast32_t N, int_fast32_t K, const float* 
  * weight matrix is column-major K x N, i.e. one output channel per row of an
  * [N, K] array, tensors are dense and do not alias, sizes are >= 1, pointers are
  * host or device memory and aligned to their element.  bool / enum arguments by value.
+ * Device operands whose rows do not start on 16 bytes are read by the aligned 16-byte
+ * vectors that hold them, so up to 15 bytes in front of and behind such an operand are
+ * read, in the same allocation, and ignored; nothing outside a result is written.
  * A call whose operands are all device memory only enqueues and may be captured
  * into a CUDA graph; a call with host operands on a capturing stream is refused
  * (EXO_B200_ERR_UNSUPPORTED).  A matrix operand of a product whose base or whose
@@ -243,7 +246,8 @@ void linear_i8_bf16_exo( void *ctxt, int_fast32_t M, int_fast32_t N, int_fast32_
 void linear_i8_f32_exo( void *ctxt, int_fast32_t M, int_fast32_t N, int_fast32_t K, const float* X, const int8_t* B, const float* col_scale, const float* bias, int8_t* Q, float* row_scale, float* Y );
 
 /* Activations of the gated projections: g / (1 + exp(-g)); g Phi(g); and Phi's tanh approximation
- * g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))). */
+ * g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))).  In fp32 each is within 2^-13 of its value, the negative tail
+ * included, as long as its factor of g is above 2^-126 (below, it is zero). */
 enum { EXO_B200_ACT_SILU = 0, EXO_B200_ACT_GELU = 1, EXO_B200_ACT_GELU_TANH = 2 };
 
 /* gated_bf16_exo: H = act(G) * U with G = X Wg^T, U = X Wu^T in one kernel (fp32 sums; H is formed from
@@ -255,7 +259,7 @@ void gated_bf16_exo( void *ctxt, int_fast32_t activation, int_fast32_t M, int_fa
  *   dG = dH * U * act'(G), dU = dH * act(G)                     (written, bf16[M,F])
  *   dX = dG Wg + dU Wu : bf16[M,K];  dWg = dG^T X, dWu = dU^T X : bf16[F,K]
  * dX may be NULL (not computed), and so may dWg and dWu together.  The products take dG and dU as rounded
- * to bf16; their sums are fp32 and rounded once. */
+ * to bf16; their sums are fp32 and rounded once.  A NaN in G, U or dH is one in what depends on it. */
 void gated_bf16_backward_exo( void *ctxt, int_fast32_t activation, int_fast32_t M, int_fast32_t F, int_fast32_t K, const uint16_t* X, const uint16_t* Wg, const uint16_t* Wu, const uint16_t* G, const uint16_t* U, const uint16_t* dH, uint16_t* dG, uint16_t* dU, uint16_t* dX, uint16_t* dWg, uint16_t* dWu );
 
 /* gated_i8_bf16_exo: gated_bf16_exo on quantised operands: G = (A Bg^T) * row_scale * gate_scale,
