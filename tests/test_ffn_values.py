@@ -160,3 +160,79 @@ def test_gates_that_are_not_finite(lib, act):
         got = widen(h.cpu().numpy().view(np.uint16))
         assert np.isnan(got[0]).all() and (got[1] == np.inf).all() and np.isfinite(got[3:]).all()
         assert (np.isnan(got[2]) | (got[2] == 0)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M", [3, 20, 300])
+def test_gated_i8_with_scales_that_are_not_finite(lib, act, M):
+    """A row that could not be quantised has scale NaN: its row of H is NaN and no other; so is the column of a channel
+    whose scale is NaN, and a gate that overflows to infinity gives what infinity gives."""
+    import torch
+
+    F, K = 200, 96
+    one = torch.ones(M, K, dtype=torch.int8, device="cuda")
+    w = torch.ones(F, K, dtype=torch.int8, device="cuda")
+    row, gate, up = torch.full((M,), 0.01, device="cuda"), torch.ones(F, device="cuda"), torch.ones(F, device="cuda")
+    row[1], gate[5], up[7], gate[9] = math.nan, math.nan, math.nan, math.inf
+    h = torch.zeros(M, F, dtype=torch.bfloat16, device="cuda")
+    lib.gated_i8_bf16_exo(None, ACTS[act], M, F, K, one, w, w, row, gate, up, h)
+    got = h.float().cpu().numpy()
+    bad = np.zeros((M, F), bool)
+    bad[1] = bad[:, 5] = bad[:, 7] = True
+    inf = np.zeros((M, F), bool)
+    inf[:, 9] = ~bad[:, 9]
+    assert np.isnan(got[bad]).all() and (got[inf] == np.inf).all() and np.isfinite(got[~bad & ~inf]).all()
+
+
+# ------------------------------------------------------------------ offsets beyond 32 bits
+@pytest.mark.gpu
+@pytest.mark.parametrize("F", [33000, 33001])  # rows that TMA reads and stores, and rows that are copied and stored singly
+def test_gated_tensors_beyond_32_bits(lib, F):
+    """More than 2^31 elements in H, G, U and their gradients; rows at both ends and around the border, in float64."""
+    import torch
+
+    M, K = 66000, 24
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GB")
+    g = torch.Generator(device="cuda").manual_seed(F)
+    make = lambda *s, std=1.0: torch.randn(s, generator=g, device="cuda").mul_(std).bfloat16()
+    x, wg, wu = make(M, K), make(F, K, std=0.2), make(F, K, std=0.2)
+    h, pre, up = (torch.empty(M, F, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    lib.gated_bf16_exo(None, fo.SILU, M, F, K, x, wg, wu, h, pre, up)
+    border = 2 ** 31 // F
+    rows = torch.tensor([0, 1, border - 1, border, border + 1, M - 1], device="cuda")
+    half = lambda y, err: err * (1 + fo.U16) + fo.U16 * y.abs() + fo.TINY16
+
+    def near(got, want, bound):
+        bad = ~((got.double() - want).abs() <= bound)
+        assert not bool(bad.any()), (int(bad.sum()), got[bad][:4], want[bad][:4])
+
+    xr, wgd, wud = x[rows].double(), wg.double(), wu.double()
+    wantg, wantu = xr @ wgd.T, xr @ wud.T
+    eg, eu = (fo.sum_slack(K) * (xr.abs() @ w.abs().T) for w in (wgd, wud))
+    near(pre[rows], wantg, half(wantg, eg))
+    near(up[rows], wantu, half(wantu, eu))
+    a = wantg * torch.sigmoid(wantg)
+    ea = 1.2 * eg + TAIL * a.abs()
+    near(h[rows], a * wantu, half(a * wantu, ea * wantu.abs() + a.abs() * eu + ea * eu + 2 * fo.U32 * (a * wantu).abs()))
+    # the backward pass, with H as the gradient of itself
+    dg, du = (torch.empty(M, F, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    dx, dwg, dwu = (torch.empty(s, dtype=torch.bfloat16, device="cuda") for s in ((M, K), (F, K), (F, K)))
+    lib.gated_bf16_backward_exo(None, fo.SILU, M, F, K, x, wg, wu, pre, up, h, dg, du, dx, dwg, dwu)
+    gr, ur, hr = (t[rows].double() for t in (pre, up, h))
+    p = torch.sigmoid(gr)
+    slope = p + gr * p * (1 - p)
+    near(dg[rows], hr * ur * slope, half(hr * ur * slope, (hr * ur).abs() * TAIL * p * (1 + gr.abs())))
+    near(du[rows], hr * gr * p, half(hr * gr * p, TAIL * (hr * gr * p).abs()))
+    # the products take dG and dU as the library rounded them
+    dgr, dur = dg[rows].double(), du[rows].double()
+    want = dgr @ wgd + dur @ wud
+    near(dx[rows], want, half(want, fo.sum_slack(2 * F) * (dgr.abs() @ wgd.abs() + dur.abs() @ wud.abs())))
+    cols, xd = torch.tensor([0, 1, F // 2, F - 1], device="cuda"), x.double()
+    for got, d in ((dwg, dg), (dwu, du)):
+        d = d[:, cols].double().T
+        near(got[cols], d @ xd, half(d @ xd, fo.sum_slack(M) * (d.abs() @ xd.abs())))
+    del h, pre, up, dg, du
+    lib.trim()
+    torch.cuda.empty_cache()
