@@ -269,7 +269,7 @@ class Context:
     handle = None
 
     def __init__(self, device: int = -1, stream: int | None = None, sgemm_path: int = SGEMM_FFMA):
-        self.lock = threading.Lock()  # held while a thread sets the stream and makes its call
+        self.lock = threading.RLock()  # held while a thread sets the stream and makes its call (a finaliser may call, too)
         self._dll = _lib.load()
         self.handle = self._dll.exo_b200_context_create(device, stream)
         if not self.handle:
