@@ -106,8 +106,7 @@ def build_call(force: bool = False) -> "str | None":
         return CALL
 
     def without(why):
-        sys.stderr.write(f"exo_b200: the binding's fast path is not built ({why}); calls go through the interpreter\n")
-        _remove(CALL)
+        sys.stderr.write(f"exo_b200: the binding's fast path is not built ({why})\n")
 
     headers = sysconfig.get_paths()["include"]
     if not os.path.exists(os.path.join(headers, "Python.h")):

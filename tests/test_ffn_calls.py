@@ -197,6 +197,10 @@ def test_no_compiler_is_no_error_and_leaves_no_old_module(call_at, monkeypatch, 
     os.utime(build.CALL, (1, 1))
     assert build.build_call() is None
     assert os.listdir(path) == [] and "fast path is not built" in capsys.readouterr().err
+    with open(build.CALL, "wb") as f:
+        f.write(b"of this source")
+    assert build.build_call(force=True) is None  # one that is up to date stays
+    assert os.listdir(path) == [os.path.basename(build.CALL)]
 
 
 def test_no_headers_is_no_error_and_leaves_no_old_module(call_at, monkeypatch):
