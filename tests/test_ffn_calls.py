@@ -95,7 +95,7 @@ def test_graphs_with_copies_run_beside_one_another(lib):
         with torch.cuda.graph(graph):
             lib.gated_bf16_exo(None, 1, M, F, K, xi, wg, wu, g, None, None)
         graphs.append(graph)
-    for round in range(10):
+    for turn in range(10):
         for g in (*got, other):
             g.zero_()
         torch.cuda.synchronize()
@@ -105,11 +105,11 @@ def test_graphs_with_copies_run_beside_one_another(lib):
                     graph.replay()
             with torch.cuda.stream(streams[2]):
                 lib.gated_bf16_exo(None, 1, 300, 2000, 519, *big, other, None, None)
-        if round % 3 == 1:
+        if turn % 3 == 1:
             lib.trim()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(other, other_want)
-        if round % 3 == 2:
+        if turn % 3 == 2:
             lib.trim()
 
 
